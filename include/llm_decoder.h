@@ -37,7 +37,14 @@ enum llm_status {
 /* Element types.  KV pools may be any of the four (the T of
  * AttentionCUDA::forward, attention/attention_cuda.cu:58-94: __half, bf16,
  * int8_t (raw values, no scale), float); weights are LLM_I8 or LLM_F16. */
-enum llm_dtype { LLM_F16 = 0, LLM_I8 = 1, LLM_F32 = 2, LLM_BF16 = 3 };
+enum llm_dtype {
+  LLM_F16 = 0,
+  LLM_I8 = 1,
+  LLM_F32 = 2,
+  LLM_BF16 = 3,
+  LLM_E4M3 = 4 /* 8-bit floats of 4 exponent and 3 mantissa bits, no infinities (OCP): pools
+                  with scales alone (kv_quant_write, kv_quant_read, pa_tree) */
+};
 enum llm_act { LLM_ACT_NONE = 0, LLM_ACT_RELU = 1, LLM_ACT_GELU = 2 };
 
 const char* llm_last_error(void);
@@ -197,6 +204,82 @@ int pa_decode_ex(const pa_kv_view* kv, const float* q, float* out, const int32_t
                  void* stream);
 
 /* ------------------------------------------------------------------------ */
+/* Quantised pages and drafted tokens                                        */
+/*                                                                           */
+/* A batch here is B rows of up to N tokens, [B][N] in every array of tokens:  */
+/* row b's token j is at position starts[b] + j (pa_tree: context_lens[b] + j) */
+/* of page-table row beam_ids[b] (NULL: b), for j < lens[b] (NULL: N; values    */
+/* outside 0 .. N are read as the nearest of the two).                          */
+/* ------------------------------------------------------------------------ */
+
+/* Scales of a view whose pools are quantised (kv_dtype LLM_I8 or LLM_E4M3): one
+ * fp32 for every page slot, so one for each token and head.  An element's value
+ * is its code times its row's scale. */
+typedef struct pa_kv_scales {
+  float* k_scale;      /* [num_pages][page_size] fp32, device */
+  float* v_scale;      /* same layout */
+  int64_t page_stride; /* floats from page p to page p + 1; 0 = page_size */
+} pa_kv_scales;
+
+/* Quantise K and V of new tokens into their pages: k, v [B][N][H][D] of dtype
+ * (LLM_F32, LLM_F16 or LLM_BF16), H = kv->num_heads, D = kv->head_dim, with
+ * token_stride elements from token to token (0: H*D).  For a row x of D
+ * elements with a = max |x|:
+ *   LLM_I8    scale = a / 127, code = 127 x / a to the nearest whole number
+ *   LLM_E4M3  scale = a / 448, code = 448 x / a to the nearest of the type
+ * (codes as if in exact arithmetic, halves to the even one; scales rounded to
+ * fp32; a = 0: scale and codes 0).  A row with an infinity or a NaN gets the
+ * scale NaN and codes 0.  A token whose position is negative or has no page is
+ * left out, as is one whose beam id the page table does not have.  Where rows of
+ * one beam overlap, the later row's token is kept.  Pages that two heads or
+ * beams share are the caller's to part before they are written (as
+ * kv_cache_fork's are by its copy-on-write).
+ * head_dim a multiple of 8 up to 256; pools, k and v 16-byte aligned, and
+ * token_stride a multiple of 16 bytes.  B <= 65535. */
+int kv_quant_write(const pa_kv_view* kv, const pa_kv_scales* scales, const void* k, const void* v,
+                   int dtype, long long token_stride, const int32_t* beam_ids,
+                   const int32_t* starts, const int32_t* lens, int B, int N, void* stream);
+
+/* Read K and V of B x N tokens back, k, v as above (written): code * scale,
+ * rounded to dtype; 0 where a position has no page or the beam id no row.
+ * Tokens j >= lens[b] are left as they were. */
+int kv_quant_read(const pa_kv_view* kv, const pa_kv_scales* scales, void* k, void* v, int dtype,
+                  long long token_stride, const int32_t* beam_ids, const int32_t* starts,
+                  const int32_t* lens, int B, int N, void* stream);
+
+/* Attention of drafted tokens over a paged cache.  Row b has context_lens[b]
+ * committed tokens (NULL: T) and N drafted ones, whose K and V are in its pages
+ * right behind them.  A drafted token sees every committed token, and drafted
+ * token j where bit j of its mask is set:
+ *   tree_mask [B][N][ceil(N / 32)] uint32, bit j % 32 of word j / 32 (its own bit
+ *   set by the caller as well); NULL: a chain, token i sees drafted 0 .. i
+ *   s_t = (q[b,i,h] . k_t) * sm_scale over the tokens that it sees
+ *   out[b,i,h] = sum_t exp(s_t - max s) v_t / (sum_t exp(s_t - max s) + 1e-6)
+ * with pa_decode's treatment of pages that are missing (masked); a token that
+ * sees nothing gets 0.  What a token does not see has no part in its result,
+ * whatever it holds.  q, out [B][N][H][D] of dtype (LLM_F32, LLM_F16 or
+ * LLM_BF16), q_stride / out_stride elements from token to token (0: H*D).
+ * H is a multiple of kv->num_heads: query head h reads the pages of head
+ * h / (H / num_heads).  Drafted tokens j >= tree_lens[b] are neither seen nor
+ * computed, and their outputs left as they were.  N = 1 is the step of single
+ * tokens (context_lens then counts the tokens ahead of it).
+ * kv->kv_dtype LLM_F16 or LLM_BF16 (scales NULL), LLM_I8 (scales NULL: raw
+ * values) or LLM_E4M3 with scales; D 64, 128 or 256; page_size a multiple of
+ * 16; N <= 1024; H / num_heads <= 64; rows of q and out 16-byte aligned.  T is a
+ * bound on the committed tokens that sizes the launch; longer contexts are read
+ * in full all the same.
+ * Scores, sums and the output are accumulated in fp32 (subnormal elements of fp16
+ * pools count as 0).  The workspace holds the
+ * parts of long rows: pa_tree_workspace_bytes, 16-byte aligned, one for each
+ * call that may run at the same time. */
+size_t pa_tree_workspace_bytes(const pa_kv_view* kv, int B, int N, int H, int T);
+int pa_tree(const pa_kv_view* kv, const pa_kv_scales* scales, const void* q, long long q_stride,
+            void* out, long long out_stride, int dtype, const int32_t* beam_ids,
+            const int32_t* context_lens, const uint32_t* tree_mask, const int32_t* tree_lens, int B,
+            int N, int H, int D, int T, float sm_scale, void* workspace, size_t workspace_bytes,
+            void* stream);
+
+/* ------------------------------------------------------------------------ */
 /* INT8 / FP16 weight GEMMs (MFMA)                                          */
 /* ------------------------------------------------------------------------ */
 
@@ -258,6 +341,41 @@ int sample_rows(const float* logits, int rows, int V, float temperature, int top
 /* The uniform draw sample_rows uses for (seed, row, counter): splitmix64 of
  * seed ^ (row << 32) ^ counter, top 24 bits / 2^24. */
 float sample_uniform_host(uint64_t seed, int row, int counter);
+
+/* What a program's requests ask of their logits before a token is chosen.  All
+ * arrays are device memory; NULL: without. */
+typedef struct logits_rules {
+  const int32_t* history;      /* [rows] of history_len token ids; ids outside 0 .. V - 1 are skipped */
+  long long history_stride;    /* ids from row to row; 0: one list for all rows */
+  int history_len;
+  const int32_t* history_lens; /* [rows] ids that the row has (NULL: history_len) */
+  const int32_t* prompt_lens;  /* [rows] the first of them that the model was given (NULL: 0) */
+  const float* repetition;     /* [rows], > 0; 1 = off */
+  const float* frequency;      /* [rows]; 0 = off */
+  const float* presence;       /* [rows]; 0 = off */
+  const int32_t* bias_ids;     /* [rows] of bias_len ids; those outside 0 .. V - 1 are skipped */
+  const float* bias;           /* their biases; of an id's entries in a row the last counts */
+  long long bias_stride;       /* entries from row to row; 0: one list for all rows */
+  int bias_len;
+  const uint32_t* allowed;     /* [num_masks][ceil(V / 32)]: bit v % 32 of word v / 32 set: allowed */
+  int num_masks;
+  const int32_t* allowed_rows; /* [rows] the row's mask, none for numbers outside 0 .. num_masks - 1
+                                  (NULL: mask r for row r) */
+} logits_rules;
+
+/* Penalties for repeated tokens, biases and grammar masks, one pass over logits
+ * [rows][V] of dtype (LLM_F32, LLM_F16 or LLM_BF16), `stride` elements from row
+ * to row (0: V), into out of the same layout (out == logits: in place; other
+ * overlaps are not allowed).  With c the times that token v is in its row's
+ * history behind the prompt and p whether it is in the prompt:
+ *   x = logits[r][v]
+ *   c > 0 or p:  x = x > 0 ? x / repetition : x * repetition
+ *   x = x - (frequency * c + presence * [c > 0])
+ *   x = x + bias
+ *   not allowed: x = -infinity
+ * in fp32, rounded once at the end.  rows <= 65535. */
+int logits_adjust(const void* logits, void* out, int dtype, int rows, int V, long long stride,
+                  const logits_rules* rules, void* stream);
 
 /* Per-row dynamic int8 quantisation (attention_cpu/int8_quant.cpp:5-13,59-64):
  * scale_r = 127/(absmax_r + 1e-6); q = clamp(round(x*scale_r)); inv_scale[r] = 1/scale_r. */

@@ -1,0 +1,169 @@
+// pa_tree: checks, the split of long rows over workgroups, and their merge.
+#include "pa_tree.hpp"
+
+#include <algorithm>
+#include <climits>
+
+namespace llm {
+namespace {
+
+constexpr int kMergeThreads = 256;
+
+// A row's parts, relative to the largest of their maxima: D / 4 threads a row.
+__global__ __launch_bounds__(kMergeThreads) void pa_tree_merge_kernel(TreeArgs a, int d4_log) {
+  const long long row = (long long)blockIdx.x * (kMergeThreads >> d4_log) + (threadIdx.x >> d4_log);
+  const int d = (threadIdx.x & ((1 << d4_log) - 1)) * 4, D = 4 << d4_log;
+  if (row >= (long long)a.B * a.N * a.H) return;
+  const long long token = row / a.H;
+  const int h = (int)(row - token * a.H), b = (int)(token / a.N), i = (int)(token - (long long)b * a.N);
+  const TreeRow tr = tree_row(a, b);
+  if (i >= tr.n) return;
+  const int parts = max((tr.L + tr.split_len - 1) / tr.split_len, 1);
+  const float* ml = a.ml + (size_t)row * a.nsplit * 2;
+  const float* acc = a.acc + (size_t)row * a.nsplit * D + d;
+  float M = kNegSentinel;
+  for (int s = 0; s < parts; ++s) M = fmaxf(M, ml[2 * s]);
+  float sum = 0.f;
+  f32x4 x = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < parts; ++s) {
+    const float weight = __builtin_amdgcn_exp2f(ml[2 * s] - M);
+    sum = fmaf(ml[2 * s + 1], weight, sum);
+    x += *reinterpret_cast<const f32x4*>(acc + (size_t)s * D) * weight;
+  }
+  x *= 1.f / (sum + 1e-6f);
+  const size_t at = (size_t)token * a.out_stride + (size_t)h * D + d;
+  if (a.dtype == LLM_F32) {
+    *reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + at) = x;
+  } else if (a.dtype == LLM_F16) {
+    typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+    *reinterpret_cast<h4*>(static_cast<_Float16*>(a.out) + at) = __builtin_convertvector(x, h4);
+  } else {
+    typedef __bf16 b4 __attribute__((ext_vector_type(4)));
+    *reinterpret_cast<b4*>(static_cast<__bf16*>(a.out) + at) = __builtin_convertvector(x, b4);
+  }
+}
+
+struct TreePlan {
+  int tiles;  // row tiles of a workgroup
+  int row_groups, nsplit, split_keys;
+};
+
+// Splits: as many as bring the launch to about 1024 workgroups, none below 256 keys (the 4
+// waves' two blocks each).
+TreePlan tree_plan(const pa_kv_view& kv, int B, int N, int H, int T) {
+  TreePlan p;
+  const int rows = N * (H / kv.num_heads);
+  p.tiles = rows <= 16 ? 1 : kTreeWaves;
+  p.row_groups = (rows + 16 * p.tiles - 1) / (16 * p.tiles);
+  const long long room = (long long)kv.max_tiles * kv.page_size;
+  const long long keys = std::max(1LL, std::min((long long)T + N, room));
+  const long long base = (long long)B * kv.num_heads * p.row_groups;
+  const long long want = std::max(1LL, 1024 / base);
+  long long per = (keys + want - 1) / want;
+  per = std::max(256LL, (per + kTreeStep - 1) / kTreeStep * kTreeStep);
+  p.split_keys = (int)std::min(per, (long long)1 << 30);
+  p.nsplit = (int)std::min((keys + per - 1) / per, 1024LL);
+  return p;
+}
+
+bool tree_sizes(const pa_kv_view& kv, int B, int N, int H, int T) {
+  return B > 0 && B <= 65535 && N > 0 && N <= 1024 && H > 0 && T >= 0 && kv.num_heads > 0 &&
+         H % kv.num_heads == 0 && H / kv.num_heads <= 64 && kv.max_tiles > 0 && kv.page_size > 0 &&
+         (long long)B * kv.num_heads <= INT32_MAX / 256;
+}
+
+}  // namespace
+}  // namespace llm
+
+using namespace llm;
+
+extern "C" size_t pa_tree_workspace_bytes(const pa_kv_view* kv, int B, int N, int H, int T) {
+  if (!kv || !tree_sizes(*kv, B, N, H, T)) return 0;
+  const TreePlan p = tree_plan(*kv, B, N, H, T);
+  return p.nsplit == 1 ? 0 : (size_t)B * N * H * p.nsplit * (kv->head_dim + 2) * sizeof(float);
+}
+
+extern "C" int pa_tree(const pa_kv_view* kv, const pa_kv_scales* scales, const void* q, long long q_stride,
+                       void* out, long long out_stride, int dtype, const int32_t* beam_ids,
+                       const int32_t* context_lens, const uint32_t* tree_mask, const int32_t* tree_lens, int B,
+                       int N, int H, int D, int T, float sm_scale, void* workspace, size_t workspace_bytes,
+                       void* stream) {
+  if (const int rc = check_paged_view("pa_tree", kv, scales)) return rc;
+  LLM_REQUIRE(B >= 0 && N >= 0 && H > 0 && D > 0 && T >= 0, "pa_tree: bad B/N/H/D/T");
+  LLM_REQUIRE(kv->head_dim == D, "pa_tree: D != kv->head_dim");
+  LLM_REQUIRE(H % kv->num_heads == 0, "pa_tree: H must be a multiple of kv->num_heads");
+  LLM_REQUIRE(value_size(dtype) > 0, "pa_tree: dtype must be LLM_F32, LLM_F16 or LLM_BF16");
+  LLM_REQUIRE(sm_scale == sm_scale && sm_scale - sm_scale == 0.f, "pa_tree: sm_scale must be finite");
+  LLM_REQUIRE(kv->kv_dtype == LLM_I8 || (kv->kv_dtype == LLM_E4M3) == (scales != nullptr),
+              "pa_tree: LLM_E4M3 pools need scales, 16-bit ones have none");
+  if (D != 64 && D != 128 && D != 256)
+    return fail(LLM_ERR_UNSUPPORTED, "pa_tree: head_dim must be 64, 128 or 256");
+  if (kv->page_size % 16 != 0)
+    return fail(LLM_ERR_UNSUPPORTED, "pa_tree: page_size must be a multiple of 16");
+  if (B == 0 || N == 0) return LLM_OK;
+  if (!tree_sizes(*kv, B, N, H, T))
+    return fail(LLM_ERR_UNSUPPORTED, "pa_tree: B <= 65535, N <= 1024, H / num_heads <= 64, "
+                                     "B * num_heads < 2^23");
+  LLM_REQUIRE(q && out, "pa_tree: q/out NULL");
+  const int es = value_size(dtype);
+  if (q_stride == 0) q_stride = (long long)H * D;
+  if (out_stride == 0) out_stride = (long long)H * D;
+  LLM_REQUIRE(q_stride >= (long long)H * D && out_stride >= (long long)H * D && q_stride * es % 16 == 0 &&
+                  out_stride * es % 16 == 0 && aligned16(q) && aligned16(out),
+              "pa_tree: rows of q and out must be 16-byte aligned, strides 0 or >= H * D");
+  const TreePlan p = tree_plan(*kv, B, N, H, T);
+  LLM_REQUIRE(p.nsplit == 1 || (workspace && aligned16(workspace) &&
+                                workspace_bytes >= pa_tree_workspace_bytes(kv, B, N, H, T)),
+              "pa_tree: workspace NULL, not 16-byte aligned or below pa_tree_workspace_bytes");
+  TreeArgs a{};
+  a.q = q;
+  a.out = out;
+  a.dtype = dtype;
+  a.q_stride = q_stride;
+  a.out_stride = out_stride;
+  a.k_pool = static_cast<const uint8_t*>(kv->k_pool);
+  a.v_pool = static_cast<const uint8_t*>(kv->v_pool);
+  if (scales) {
+    a.k_scale = scales->k_scale;
+    a.v_scale = scales->v_scale;
+    a.scale_stride = scales->page_stride ? (size_t)scales->page_stride : (size_t)kv->page_size;
+  }
+  a.page_stride = paged_stride(*kv);
+  a.table = kv->page_table;
+  a.num_pages = kv->num_pages;
+  a.num_beams = kv->num_beams;
+  a.kv_heads = kv->num_heads;
+  a.max_tiles = kv->max_tiles;
+  a.page_size = kv->page_size;
+  a.beam_ids = beam_ids;
+  a.context_lens = context_lens;
+  a.tree_lens = tree_lens;
+  a.mask = tree_mask;
+  a.mask_words = (N + 31) / 32;
+  a.B = B;
+  a.N = N;
+  a.H = H;
+  a.G = H / kv->num_heads;
+  a.T = T;
+  a.scale2 = sm_scale * kLog2e;
+  a.nsplit = p.nsplit;
+  a.split_keys = p.split_keys;
+  a.acc = static_cast<float*>(workspace);
+  a.ml = a.acc + (size_t)B * N * H * p.nsplit * D;
+  const hipStream_t st = as_stream(stream);
+  const dim3 grid(B * kv->num_heads, p.nsplit, p.row_groups);
+  hipError_t e = kv->kv_dtype == LLM_F16    ? launch_tree_f16(a, D, p.tiles, grid, st)
+                 : kv->kv_dtype == LLM_BF16 ? launch_tree_bf16(a, D, p.tiles, grid, st)
+                 : kv->kv_dtype == LLM_I8   ? launch_tree_i8(a, D, p.tiles, grid, st)
+                                            : launch_tree_e4m3(a, D, p.tiles, grid, st);
+  LLM_HIP_RET(e);
+  if (p.nsplit > 1) {
+    const int d4_log = D == 64 ? 4 : D == 128 ? 5 : 6, per = kMergeThreads >> d4_log;
+    const long long rows = (long long)B * N * H;
+    LLM_REQUIRE((rows + per - 1) / per <= INT32_MAX / 256, "pa_tree: too many rows");
+    hipLaunchKernelGGL(pa_tree_merge_kernel, dim3((unsigned)((rows + per - 1) / per)), dim3(kMergeThreads), 0, st,
+                       a, d4_log);
+    LLM_HIP_RET(hipGetLastError());
+  }
+  return LLM_OK;
+}

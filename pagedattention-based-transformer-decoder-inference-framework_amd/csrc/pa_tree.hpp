@@ -1,0 +1,81 @@
+// Attention of drafted tokens over a paged cache (pa_tree; its contract is in llm_decoder.h).
+//
+// A workgroup takes rows (tokens x heads of the group) of one key/value head and one split of
+// its keys.  Up to 16 rows are one tile, whose blocks of 32 keys its 4 waves take in turn, merged
+// through LDS; more are 4 tiles, a wave each, which read the same keys at about the same
+// time, from one L1.  All operands come from memory straight into registers, one block ahead:
+//   S^T[32 keys][16 rows] = K . Q^T       v_mfma_f32_16x16x32, two tiles of 16 keys
+//   O^T[D][16 rows]      += V^T . P^T
+// A lane (g = lane / 16, c = lane % 16) holds the scores of 8 keys (16 u + 4 g + r; u < 2,
+// r < 4) of row c, which are the B operand of the second product once its k slots are taken in
+// that order.  The A operand wants, in lane c, 8 keys of one dim: a lane loads the dims
+// c D/16 .. of its 8 keys, 2 to 32 bytes a key and whole rows together, and exchanges
+// bytes among its own registers (v_perm), so V^T needs no LDS.  Tile dd of O^T then has rows
+// m = c for the dims c D/16 + dd: lane (g, c) ends with dims 4 g D/16 .. (4 g + 4) D/16 of row c.
+//
+// 8-bit codes become fp16 on the way into the products, exactly (int8: 0x6400 | code ^ 0x80 is
+// the fp16 number 1152 + code; e4m3: one conversion for two).  A key's scale multiplies its
+// scores, a value's scale its probabilities.
+//
+// Precision: queries enter as parts of 16 bits (fp32 ones as two of fp16, three of bf16: 22 and
+// 24 bits; others exactly), probabilities as two, the rest is fp32.  The products drop fp16
+// subnormals, so a row of queries is scaled to 2^14 by a power of two, probabilities by 2^14, and
+// values' scales are taken in units of a power of two above the largest met.
+//
+// Keys that a row does not see get the score -infinity.  Their V still meets a probability of 0
+// in the product, and 0 times NaN is NaN: rows of V that nobody sees (behind the row's end, in
+// missing pages) are zeroed, and what is not a number in a drafted token's V is taken as 0;
+// if there was any, the rows that see it get their infinities and NaNs in a pass behind the others,
+// from products of ones.
+#pragma once
+
+#include "common.hpp"
+#include "paged_rows.hpp"
+
+namespace llm {
+
+struct TreeArgs {
+  const void* q;
+  void* out;
+  int dtype;
+  long long q_stride, out_stride;  // elements from token to token
+  const uint8_t *k_pool, *v_pool;
+  const float *k_scale, *v_scale;  // NULL: 1
+  size_t page_stride, scale_stride;
+  const int32_t* table;
+  int num_pages, num_beams, kv_heads, max_tiles, page_size;
+  const int32_t *beam_ids, *context_lens, *tree_lens;
+  const uint32_t* mask;
+  int mask_words;
+  int B, N, H, G, T;  // G = H / kv_heads
+  float scale2;       // sm_scale log2(e)
+  int nsplit, split_keys;
+  float *acc, *ml;  // [row][split][D], [row][split][2], row = (b N + token) H + head
+};
+
+constexpr int kTreeWaves = 4, kTreeKeys = 32;
+constexpr int kTreeStep = kTreeWaves * kTreeKeys;
+
+// Committed and all tokens of row b, its drafts, and the keys of one of its splits: nsplit of
+// them hold the row however long it is.
+struct TreeRow {
+  int n, C, L, split_len;
+};
+__device__ __forceinline__ TreeRow tree_row(const TreeArgs& a, int b) {
+  TreeRow r;
+  const int room = a.max_tiles * a.page_size;
+  r.n = a.tree_lens ? clamp_int(a.tree_lens[b], 0, a.N) : a.N;
+  r.C = clamp_int(a.context_lens ? a.context_lens[b] : a.T, 0, room);
+  r.L = min(r.C + r.n, room);
+  const int even = ((r.L + a.nsplit - 1) / a.nsplit + kTreeStep - 1) / kTreeStep * kTreeStep;
+  r.split_len = max(a.split_keys, even);
+  return r;
+}
+
+// pa_tree_*.hip
+hipError_t launch_tree_f16(const TreeArgs& a, int D, int tiles, dim3 grid, hipStream_t st);
+hipError_t launch_tree_bf16(const TreeArgs& a, int D, int tiles, dim3 grid, hipStream_t st);
+hipError_t launch_tree_i8(const TreeArgs& a, int D, int tiles, dim3 grid, hipStream_t st);
+hipError_t launch_tree_e4m3(const TreeArgs& a, int D, int tiles, dim3 grid, hipStream_t st);
+
+}  // namespace llm

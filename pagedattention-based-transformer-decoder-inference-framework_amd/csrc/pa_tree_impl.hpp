@@ -1,0 +1,589 @@
+// The kernel of pa_tree.hpp, for the files that build it for one type of pool each.
+#pragma once
+
+#include <type_traits>
+
+#include "pa_tree.hpp"
+
+namespace llm {
+namespace {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+// Operands of 16 bits, as the products of one pool type take them.
+template <bool BF>
+struct Half {  // fp16
+  static constexpr float kP = 16384.f;    // probabilities enter times this
+  static constexpr float kGrow = 1.f;     // a maximum moves when it grew by more (log2 units)
+  static constexpr uint32_t kOne = 0x3c00u;
+  static __device__ __forceinline__ f32x4 dot(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
+                                                  __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pair(float x, float y) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{x, y}, f16x2));
+  }
+  static __device__ __forceinline__ f32x2 values(uint32_t w) {
+    const f16x2 h = __builtin_bit_cast(f16x2, w);
+    return f32x2{(float)h[0], (float)h[1]};
+  }
+};
+template <>
+struct Half<true> {  // bf16
+  static constexpr float kP = 1.f;
+  static constexpr float kGrow = 8.f;
+  static constexpr uint32_t kOne = 0x3f80u;
+  static __device__ __forceinline__ f32x4 dot(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pair(float x, float y) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{x, y}, bf16x2));
+  }
+  static __device__ __forceinline__ f32x2 values(uint32_t w) {
+    return f32x2{__builtin_bit_cast(float, w << 16), __builtin_bit_cast(float, w & 0xffff0000u)};
+  }
+};
+
+// x, y as `PARTS` pairs of halves, each what the ones before it leave.
+template <typename Hf, int PARTS>
+__device__ __forceinline__ void split_parts(float x, float y, uint32_t (&w)[PARTS]) {
+#pragma unroll
+  for (int i = 0; i < PARTS; ++i) {
+    w[i] = Hf::pair(x, y);
+    if (i + 1 < PARTS) {
+      asm("" : "+v"(w[i]));  // (the compiler would convert a second time for what is left)
+      const f32x2 v = Hf::values(w[i]);
+      x -= v[0];
+      y -= v[1];
+    }
+  }
+}
+
+// Two 8-bit codes of a register (its low or high half) as fp16.
+template <int KVT, bool HIGH>
+__device__ __forceinline__ uint32_t two_codes(uint32_t w) {
+  if constexpr (KVT == LLM_I8) {  // w ^ 0x80808080 before
+    const uint32_t x = __builtin_amdgcn_perm(0x64646464u, w, HIGH ? 0x04030402u : 0x04010400u);
+    return __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, x) - f16x2{1152.f, 1152.f});
+  } else {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, HIGH));
+  }
+}
+
+template <int KVT>
+struct Raw {
+  static constexpr bool QUANT = KVT == LLM_I8 || KVT == LLM_E4M3;
+  static constexpr int ES = QUANT ? 1 : 2;
+};
+
+// An element of a pool that is not a number, as its own bits.
+template <int KVT>
+struct Unusable;
+template <>
+struct Unusable<LLM_F16> {
+  static constexpr uint32_t kInf = 0x7c00u;
+};
+template <>
+struct Unusable<LLM_BF16> {
+  static constexpr uint32_t kInf = 0x7f80u;
+};
+template <>
+struct Unusable<LLM_E4M3> {  // NaN alone
+  static constexpr uint32_t kInf = 0x7fu;
+};
+// The elements of w with 0 in the place of infinities and NaNs.
+template <int KVT>
+__device__ __forceinline__ uint32_t usable(uint32_t w) {
+  constexpr int BITS = KVT == LLM_E4M3 ? 8 : 16;
+  constexpr uint32_t kInf = Unusable<KVT>::kInf, kAll = (1u << BITS) - 1u;
+  uint32_t kept = 0;
+#pragma unroll
+  for (int s = 0; s < 32; s += BITS)
+    if ((w >> s & kInf) != kInf) kept |= w & kAll << s;
+  return kept;
+}
+
+// NQ: parts of a query; KW: waves that share a row tile's keys, the others have tiles of their own.
+template <int KVT, int D, int NQ, int KW>
+__global__ __launch_bounds__(64 * kTreeWaves, D <= 128 ? 2 : 1) void pa_tree_kernel(TreeArgs a) {
+  constexpr bool QUANT = Raw<KVT>::QUANT;
+  constexpr int ES = Raw<KVT>::ES, ROWB = D * ES;
+  using Hf = Half<KVT == LLM_BF16>;
+  constexpr int NK = D / 32;          // steps of 32 dims of q.k
+  constexpr int NKL = ROWB / 64;      // 16-byte loads of a key tile
+  constexpr int ND = D / 16;          // tiles of the output, dims of a lane's keys
+  constexpr int NV = ND * ES / 4;     // registers of them
+  constexpr int NP = 2;               // parts of a probability
+  constexpr int RW = kTreeWaves / KW; // row tiles
+  constexpr bool AHEAD = ROWB < 512;  // a block ahead of the one in work fits the registers
+  __shared__ float s_acc[kTreeWaves][16][D + 4];
+  __shared__ float s_ml[kTreeWaves][16][2];
+
+  const int lane = lane_id(), g = lane >> 4, c = lane & 15;
+  const int w = wave_id_uniform(), kw = w % KW;
+  const int pair = blockIdx.x, b = pair / a.kv_heads, kvh = pair - b * a.kv_heads;
+  const int split = blockIdx.y;
+  const TreeRow tr = tree_row(a, b);
+  const int first = blockIdx.z * 16 * RW, row0 = first + w / KW * 16;  // of the workgroup, the wave
+  const int all_rows = tr.n * a.G, rows = all_rows - row0;
+  const int lo = split * tr.split_len;
+  if (first >= all_rows || (split > 0 && lo >= tr.L)) return;
+  const int hi = min(lo + tr.split_len, tr.L);
+  const int beam = a.beam_ids ? a.beam_ids[b] : b;
+  const bool has_beam = beam >= 0 && beam < a.num_beams;
+  const int32_t* pt = a.table + ((size_t)(has_beam ? beam : 0) * a.kv_heads + kvh) * a.max_tiles;
+  const int blocks = (hi - lo + kTreeKeys - 1) / kTreeKeys;
+
+  // Lane i: the page of 16 keys, half i % 2 of this wave's block number from + i / 2 (-1: none),
+  // and where in it they begin.
+  int pages, slots;
+  auto look_up = [&](int from) {
+    const int key = lo + ((from + (lane >> 1)) * KW + kw) * kTreeKeys + 16 * (lane & 1);
+    const int tile = key / a.page_size;
+    slots = key - tile * a.page_size;
+    const int p = has_beam && key < hi ? pt[tile] : -1;
+    pages = p >= 0 && p < a.num_pages ? p : -1;
+  };
+
+  // a block's operands as they are in memory
+  struct Block {
+    u32x4 k[2][NKL];
+    uint32_t v[2][4][NV];
+    f32x4 ks[2], vs[2];
+    int page[2];
+  };
+  auto load = [&](Block& x, int i) {  // this wave's i-th block
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      x.page[u] = __builtin_amdgcn_readlane(pages, (2 * i + u) & 63);
+      const int page = max(x.page[u], 0);  // (what is read of page 0 instead is masked)
+      const int slot = __builtin_amdgcn_readlane(slots, (2 * i + u) & 63);
+      const size_t base = (size_t)page * a.page_stride + (size_t)slot * ROWB;
+      const uint8_t *kp = a.k_pool + base, *vp = a.v_pool + base;
+#pragma unroll
+      for (int l = 0; l < NKL; ++l)
+        x.k[u][l] = *reinterpret_cast<const u32x4*>(kp + (uint32_t)(c * ROWB + 64 * l + 16 * g));
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const uint8_t* at = vp + (uint32_t)((4 * g + r) * ROWB + c * ND * ES);
+        if constexpr (NV == 1) {
+          x.v[u][r][0] = *reinterpret_cast<const uint32_t*>(at);
+        } else if constexpr (NV == 2) {
+          const u32x2 y = *reinterpret_cast<const u32x2*>(at);
+          x.v[u][r][0] = y[0], x.v[u][r][1] = y[1];
+        } else {
+#pragma unroll
+          for (int o = 0; o < NV; o += 4) {
+            const u32x4 y = *reinterpret_cast<const u32x4*>(at + 4 * o);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x.v[u][r][o + e] = y[e];
+          }
+        }
+      }
+      if constexpr (QUANT) {
+        if (a.k_scale) {
+          const size_t s = (size_t)page * a.scale_stride + slot;
+          const float *ks = a.k_scale + s, *vs = a.v_scale + s;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            x.ks[u][r] = ks[4 * g + r];
+            x.vs[u][r] = vs[4 * g + r];
+          }
+        } else {
+          x.ks[u] = x.vs[u] = f32x4{1.f, 1.f, 1.f, 1.f};
+        }
+      }
+    }
+  };
+
+  // Queries: lane (g, c) holds row c's dims, those of the 16 bytes of K that it loads.
+  u32x4 q[NQ][NK];
+  float qf = fmaxf(fabsf(a.scale2), 1e-37f);  // what its scores are multiplied by, in log2 units: > 0, so
+                                              // that -infinity stays what it is
+  const int tok = (row0 + (c < rows ? c : 0)) / a.G;
+  {
+    const bool ok = c < rows;
+    const int h = kvh * a.G + row0 + (ok ? c : 0) - tok * a.G;
+    const size_t at = ((size_t)b * a.N + (ok ? tok : 0)) * a.q_stride + (size_t)(ok ? h : 0) * D;
+    float x[NK][8];
+    float most = 0.f;
+#pragma unroll
+    for (int kk = 0; kk < NK; ++kk) {
+      const int d = ES == 1 ? 64 * (kk / 2) + 16 * g + 8 * (kk & 1) : 32 * kk + 8 * g;
+      if (a.dtype == LLM_F32) {
+        const float* p = static_cast<const float*>(a.q) + at + d;
+        const f32x4 y = *reinterpret_cast<const f32x4*>(p), z = *reinterpret_cast<const f32x4*>(p + 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[kk][e] = y[e], x[kk][4 + e] = z[e];
+      } else {
+        const u32x4 y = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q) + at + d);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const f32x2 z = a.dtype == LLM_F16 ? Half<false>::values(y[e]) : Half<true>::values(y[e]);
+          x[kk][2 * e] = z[0], x[kk][2 * e + 1] = z[1];
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if (!ok) x[kk][e] = 0.f;
+        if (a.scale2 < 0.f) x[kk][e] = -x[kk][e];
+        most = fmaxf(most, fabsf(x[kk][e]));
+      }
+    }
+    if constexpr (KVT != LLM_BF16) {
+      int e = 0;
+      (void)frexpf(rows_max(most), &e);  // most < 2^e
+      e = clamp_int(e, -100, 100);
+      const float up = ldexpf(1.f, 14 - e);
+      qf = fmaxf(qf * ldexpf(1.f, e - 14), 1e-37f);
+#pragma unroll
+      for (int kk = 0; kk < NK; ++kk)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[kk][i] *= up;
+    }
+#pragma unroll
+    for (int kk = 0; kk < NK; ++kk)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t part[NQ];
+        split_parts<Hf, NQ>(x[kk][2 * i], x[kk][2 * i + 1], part);
+#pragma unroll
+        for (int p = 0; p < NQ; ++p) q[p][kk][i] = part[p];
+      }
+  }
+
+  f32x4 o[ND];
+  // what p is relative to, the maximum (m <= top <= m + kGrow), the sum
+  float m = kNegSentinel, top = kNegSentinel, l = 0.f;
+  float unit = 0x1p-100f;  // of the values' scales: a power of two, at least the largest met
+#pragma unroll
+  for (int dd = 0; dd < ND; ++dd) o[dd] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  // Keys key0 .. key0 + 31 that a drafted token sees, as far as its mask says.
+  auto visible = [&](int token, int key0) -> uint32_t {
+    const int j0 = key0 - tr.C;  // drafted token of the first key
+    if (j0 <= -32) return 0xffffffffu;
+    if (!a.mask) {
+      const int k = token - j0;  // the last key it sees
+      return k >= 31 ? 0xffffffffu : k < 0 ? 0u : (2u << k) - 1u;
+    }
+    const uint32_t* mask = a.mask + ((size_t)b * a.N + token) * a.mask_words;
+    if (j0 < 0) return mask[0] << -j0 | ((1u << -j0) - 1u);
+    const int at = j0 >> 5, sh = j0 & 31;
+    const uint32_t w0 = at < a.mask_words ? mask[at] : 0u;
+    const uint32_t w1 = at + 1 < a.mask_words ? mask[at + 1] : 0u;
+    return sh ? w0 >> sh | w1 << (32 - sh) : w0;
+  };
+  // ... and those of them that anyone may: with a page, ahead of the row's end.
+  auto present_of = [&](const int (&page)[2], int key0) -> uint32_t {
+    uint32_t present = 0xffffffffu;
+    if (page[0] < 0) present &= 0xffff0000u;
+    if (page[1] < 0) present &= 0x0000ffffu;
+    if (tr.L - key0 < 32) present &= (1u << (tr.L - key0)) - 1u;
+    return present;
+  };
+  bool unusable = false;  // a drafted token's V has held infinities or NaNs
+
+  auto attend = [&](Block& x, int i) {
+    const int key0 = lo + (i * KW + kw) * kTreeKeys;
+    const bool special = key0 + kTreeKeys > tr.C || x.page[0] < 0 || x.page[1] < 0;
+    uint32_t present = 0xffffffffu;
+    if (special) {
+      present = present_of(x.page, key0);
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const bool ok = present >> (16 * u + 4 * g + r) & 1u;
+#pragma unroll
+          for (int e = 0; e < NV; ++e) x.v[u][r][e] = ok ? x.v[u][r][e] : 0u;
+          if constexpr (QUANT) x.vs[u][r] = ok ? x.vs[u][r] : 0.f;
+        }
+      if constexpr (KVT != LLM_I8)
+        if (key0 + kTreeKeys > tr.C) {
+          bool all = true;
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+              for (int e = 0; e < NV; ++e) {
+                const uint32_t kept = usable<KVT>(x.v[u][r][e]);
+                all &= kept == x.v[u][r][e];
+                x.v[u][r][e] = kept;
+              }
+          unusable |= !all;
+        }
+    }
+    // V^T: the 8 keys' dims exchanged to 8 keys of one dim
+    u32x4 vf[ND];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf)  // keys 2 hf, 2 hf + 1 of the four
+#pragma unroll
+        for (int e = 0; e < NV; ++e) {
+          const uint32_t v0 = x.v[u][2 * hf][e], v1 = x.v[u][2 * hf + 1][e];
+          if constexpr (QUANT) {
+            const uint32_t flip = KVT == LLM_I8 ? 0x80808080u : 0u;
+            const uint32_t lo2 = __builtin_amdgcn_perm(v1, v0, 0x05010400u) ^ flip;
+            const uint32_t hi2 = __builtin_amdgcn_perm(v1, v0, 0x07030602u) ^ flip;
+            vf[4 * e][2 * u + hf] = two_codes<KVT, false>(lo2);
+            vf[4 * e + 1][2 * u + hf] = two_codes<KVT, true>(lo2);
+            vf[4 * e + 2][2 * u + hf] = two_codes<KVT, false>(hi2);
+            vf[4 * e + 3][2 * u + hf] = two_codes<KVT, true>(hi2);
+          } else {
+            vf[2 * e][2 * u + hf] = __builtin_amdgcn_perm(v1, v0, 0x05040100u);
+            vf[2 * e + 1][2 * u + hf] = __builtin_amdgcn_perm(v1, v0, 0x07060302u);
+          }
+        }
+    u32x4 kf[2][NK];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int kk = 0; kk < NK; ++kk) {
+        if constexpr (QUANT) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t y = x.k[u][kk / 2][2 * (kk & 1) + e] ^ (KVT == LLM_I8 ? 0x80808080u : 0u);
+            kf[u][kk][2 * e] = two_codes<KVT, false>(y);
+            kf[u][kk][2 * e + 1] = two_codes<KVT, true>(y);
+          }
+        } else {
+          kf[u][kk] = x.k[u][kk];
+        }
+      }
+    if constexpr (QUANT) {
+      float most = 0.f;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float s = fabsf(x.vs[u][r]);
+          if (s < INFINITY) most = fmaxf(most, s);
+        }
+      if (__any(most > unit)) {
+        int e = 0;
+        (void)frexpf(rows_max(most), &e);
+        const float next = ldexpf(1.f, min(e, 126)), down = unit / next;
+#pragma unroll
+        for (int dd = 0; dd < ND; ++dd) o[dd] *= down;
+        unit = next;
+      }
+    }
+    const float per_unit = QUANT ? Hf::kP / unit : Hf::kP;
+    f32x4 s[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int p = 0; p < NQ; ++p)
+#pragma unroll
+        for (int kk = 0; kk < NK; ++kk) s[u] = Hf::dot(kf[u][kk], q[p][kk], s[u]);
+      if constexpr (QUANT) s[u] *= x.ks[u];
+    }
+    uint32_t seen = present;
+    if (special) {
+      seen &= visible(tok, key0);
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (!(seen >> (16 * u + 4 * g + r) & 1u)) s[u][r] = -INFINITY;
+    }
+    float most = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) most = fmaxf(most, s[u][r]);
+    most = rows_max(most) * qf;
+    top = fmaxf(top, most);
+    if (__any(most > m + Hf::kGrow)) {
+      const float corr = __builtin_amdgcn_exp2f(m - top);
+      l *= corr;
+#pragma unroll
+      for (int dd = 0; dd < ND; ++dd) o[dd] *= corr;
+      m = top;
+    }
+    u32x4 ph[NP];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        float p[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int r = 2 * hf + e;
+          p[e] = __builtin_amdgcn_exp2f(fmaf(s[u][r], qf, -m));
+          l += p[e];
+          if constexpr (QUANT) {
+            p[e] *= x.vs[u][r] * per_unit;
+            if (special && !(seen >> (16 * u + 4 * g + r) & 1u)) p[e] = 0.f;  // (the scale may be NaN)
+          } else {
+            p[e] *= per_unit;
+          }
+        }
+        uint32_t part[NP];
+        split_parts<Hf, NP>(p[0], p[1], part);
+#pragma unroll
+        for (int i = 0; i < NP; ++i) ph[i][2 * u + hf] = part[i];
+      }
+#pragma unroll
+    for (int dd = 0; dd < ND; ++dd)
+#pragma unroll
+      for (int i = 0; i < NP; ++i) o[dd] = Hf::dot(vf[dd], ph[i], o[dd]);
+  };
+
+  const int mine = rows > 0 && blocks > kw ? (blocks - kw + KW - 1) / KW : 0;
+  if (mine > 0) {
+    look_up(0);
+    Block x;
+    if constexpr (AHEAD) {
+      Block y;
+      load(x, 0);
+      for (int i = 0; i < mine; i += 2) {
+        if (i + 1 < mine) load(y, i + 1);
+        attend(x, i);
+        if (i + 1 >= mine) break;
+        if (i + 2 < mine) {
+          if (((i + 2) & 31) == 0) look_up(i + 2);
+          load(x, i + 2);
+        }
+        attend(y, i + 1);
+      }
+    } else {
+      for (int i = 0; i < mine; ++i) {
+        if (i && (i & 31) == 0) look_up(i);
+        load(x, i);
+        attend(x, i);
+      }
+    }
+  }
+  if constexpr (KVT != LLM_I8)
+    if (__any(unusable)) {
+      // The rows that see them get what the products left out: sums of ones count them.
+      for (int i = max((tr.C - lo) / (KW * kTreeKeys) - 1, 0); i < mine; ++i) {
+        const int key0 = lo + (i * KW + kw) * kTreeKeys;
+        if (key0 + kTreeKeys <= tr.C) continue;
+        look_up(i);
+        const int page[2] = {__builtin_amdgcn_readlane(pages, 0), __builtin_amdgcn_readlane(pages, 1)};
+        const uint32_t present = present_of(page, key0);
+        const uint32_t seen = present & visible(tok, key0);
+        u32x4 one;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t two = seen >> (16 * (e / 2) + 4 * g + 2 * (e % 2));
+          one[e] = (two & 1u ? Hf::kOne : 0u) | (two & 2u ? Hf::kOne << 16 : 0u);
+        }
+#pragma unroll
+        for (int dd = 0; dd < ND; ++dd) {
+          u32x4 plus, minus;  // +infinity or NaN, -infinity or NaN
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            plus[e] = minus[e] = 0;
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+              const int u = e / 2, key = 4 * g + 2 * (e % 2) + s;
+              if (!(present >> (16 * u + key) & 1u)) continue;
+              const uint8_t* at = a.v_pool + (size_t)page[u] * a.page_stride +
+                                  (size_t)(__builtin_amdgcn_readlane(slots, u) + key) * ROWB + (c * ND + dd) * ES;
+              const uint32_t x = ES == 1 ? *at : *reinterpret_cast<const uint16_t*>(at);
+              constexpr uint32_t kInf = Unusable<KVT>::kInf, kSign = ES == 1 ? 0x80u : 0x8000u;
+              const bool bad = (x & kInf) == kInf, nan = ES == 1 ? bad : (x & (kSign - 1u)) > kInf;
+              if (bad && (nan || !(x & kSign))) plus[e] |= Hf::kOne << 16 * s;
+              if (bad && (nan || (x & kSign))) minus[e] |= Hf::kOne << 16 * s;
+            }
+          }
+          const f32x4 none = {0.f, 0.f, 0.f, 0.f};
+          const f32x4 up = Hf::dot(plus, one, none), down = Hf::dot(minus, one, none);
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            o[dd][r] += (up[r] > 0.f ? INFINITY : 0.f) - (down[r] > 0.f ? INFINITY : 0.f);
+        }
+      }
+    }
+
+  // The sums of a tile's waves, relative to the largest maximum of the row.
+  const float back = __builtin_amdgcn_exp2f(m - top);
+  const float sum = add(with_lane32(add(with_lane16(l * back))));
+  const float f = back * (QUANT ? unit / Hf::kP : 1.f / Hf::kP);
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+#pragma unroll
+    for (int dd = 0; dd < ND; dd += 4)
+      *reinterpret_cast<f32x4*>(&s_acc[w][c][(4 * g + r) * ND + dd]) =
+          f32x4{o[dd][r] * f, o[dd + 1][r] * f, o[dd + 2][r] * f, o[dd + 3][r] * f};
+  if (g == 0) {
+    s_ml[w][c][0] = top;
+    s_ml[w][c][1] = sum;
+  }
+  __syncthreads();
+  const int rr = threadIdx.x >> 4, part = threadIdx.x & 15;  // a row, ND of its dims
+#pragma unroll
+  for (int tile = 0; tile < RW; ++tile) {
+    const int row = first + 16 * tile + rr;
+    if (row >= all_rows) break;
+    float M = kNegSentinel;
+#pragma unroll
+    for (int v = tile * KW; v < tile * KW + KW; ++v) M = fmaxf(M, s_ml[v][rr][0]);
+    float all = 0.f, r[ND] = {};
+#pragma unroll
+    for (int v = tile * KW; v < tile * KW + KW; ++v) {
+      const float weight = __builtin_amdgcn_exp2f(s_ml[v][rr][0] - M);
+      all = fmaf(s_ml[v][rr][1], weight, all);
+#pragma unroll
+      for (int e = 0; e < ND; ++e) r[e] = fmaf(s_acc[v][rr][part * ND + e], weight, r[e]);
+    }
+    const int token = row / a.G, h = kvh * a.G + row - token * a.G;
+    if (a.nsplit > 1) {
+      const size_t at = (((size_t)b * a.N + token) * a.H + h) * a.nsplit + split;
+#pragma unroll
+      for (int e = 0; e < ND; e += 4)
+        *reinterpret_cast<f32x4*>(a.acc + at * D + part * ND + e) = f32x4{r[e], r[e + 1], r[e + 2], r[e + 3]};
+      if (part == 0) {
+        a.ml[2 * at] = M;
+        a.ml[2 * at + 1] = all;
+      }
+    } else {
+      const float inv = 1.f / (all + 1e-6f);
+      const size_t at = ((size_t)b * a.N + token) * a.out_stride + (size_t)h * D + part * ND;
+#pragma unroll
+      for (int e = 0; e < ND; e += 4) {
+        const f32x4 y = f32x4{r[e], r[e + 1], r[e + 2], r[e + 3]} * inv;
+        if (a.dtype == LLM_F32)
+          *reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + at + e) = y;
+        else
+          *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(a.out) + at + e) =
+              a.dtype == LLM_F16 ? u32x2{Half<false>::pair(y[0], y[1]), Half<false>::pair(y[2], y[3])}
+                                 : u32x2{Half<true>::pair(y[0], y[1]), Half<true>::pair(y[2], y[3])};
+      }
+    }
+  }
+}
+
+template <int KVT, int D, int NQ>
+hipError_t launch_tree_tiles(const TreeArgs& a, int tiles, dim3 grid, hipStream_t st) {
+  hipLaunchKernelGGL((tiles == 1 ? pa_tree_kernel<KVT, D, NQ, kTreeWaves> : pa_tree_kernel<KVT, D, NQ, 1>), grid,
+                     dim3(64 * kTreeWaves), 0, st, a);
+  return hipGetLastError();
+}
+
+template <int KVT, int NQ>
+hipError_t launch_tree_dim(const TreeArgs& a, int D, int tiles, dim3 grid, hipStream_t st) {
+  return D == 64    ? launch_tree_tiles<KVT, 64, NQ>(a, tiles, grid, st)
+         : D == 128 ? launch_tree_tiles<KVT, 128, NQ>(a, tiles, grid, st)
+                    : launch_tree_tiles<KVT, 256, NQ>(a, tiles, grid, st);
+}
+
+// fp16 products: queries of 16 bits are one part, fp32 ones two.
+template <int KVT>
+hipError_t launch_tree_parts(const TreeArgs& a, int D, int tiles, dim3 grid, hipStream_t st) {
+  return a.dtype == LLM_F32 ? launch_tree_dim<KVT, 2>(a, D, tiles, grid, st)
+                            : launch_tree_dim<KVT, 1>(a, D, tiles, grid, st);
+}
+
+}  // namespace
+}  // namespace llm

@@ -21,7 +21,7 @@ TUNE_LIB_PATH = HERE / "libllm_decoder_hip_tune.so"  # `make tune`: A/B hooks, n
 
 (LLM_OK, LLM_ERR_INVALID, LLM_ERR_UNSUPPORTED, LLM_ERR_HIP, LLM_ERR_OOM, LLM_ERR_IO,
  LLM_ERR_RANGE) = range(7)
-LLM_F16, LLM_I8, LLM_F32, LLM_BF16 = 0, 1, 2, 3
+LLM_F16, LLM_I8, LLM_F32, LLM_BF16, LLM_E4M3 = 0, 1, 2, 3, 4
 LLM_ACT_NONE, LLM_ACT_RELU, LLM_ACT_GELU = 0, 1, 2
 LLM_EVICT_NONE, LLM_EVICT_LRU = 0, 1
 
@@ -43,6 +43,18 @@ class PaDecodeOptions(ctypes.Structure):
                 ("top_p", ctypes.c_float), ("eos_token", ctypes.c_int),
                 ("eos_threshold", ctypes.c_float), ("probs_out", c_void_p),
                 ("scores_out", c_void_p)]
+
+
+class PaKvScales(ctypes.Structure):
+    _fields_ = [("k_scale", c_void_p), ("v_scale", c_void_p), ("page_stride", ctypes.c_int64)]
+
+
+class LogitsRules(ctypes.Structure):
+    _fields_ = [("history", c_void_p), ("history_stride", c_ll), ("history_len", c_int),
+                ("history_lens", c_void_p), ("prompt_lens", c_void_p), ("repetition", c_void_p),
+                ("frequency", c_void_p), ("presence", c_void_p), ("bias_ids", c_void_p),
+                ("bias", c_void_p), ("bias_stride", c_ll), ("bias_len", c_int),
+                ("allowed", c_void_p), ("num_masks", c_int), ("allowed_rows", c_void_p)]
 
 
 class EngineConfig(ctypes.Structure):
@@ -87,6 +99,18 @@ _SIGS = {
     "pa_decode_ex_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
     "pa_prefill": (c_int, [ctypes.POINTER(PaKvView), c_void_p, c_int, c_void_p, c_int, c_int,
                            c_int, c_int, c_float, c_void_p, c_size_t, c_void_p]),
+    "kv_quant_write": (c_int, [ctypes.POINTER(PaKvView), ctypes.POINTER(PaKvScales), c_void_p,
+                               c_void_p, c_int, c_ll, c_void_p, c_void_p, c_void_p, c_int, c_int,
+                               c_void_p]),
+    "kv_quant_read": (c_int, [ctypes.POINTER(PaKvView), ctypes.POINTER(PaKvScales), c_void_p,
+                              c_void_p, c_int, c_ll, c_void_p, c_void_p, c_void_p, c_int, c_int,
+                              c_void_p]),
+    "pa_tree_workspace_bytes": (c_size_t, [ctypes.POINTER(PaKvView), c_int, c_int, c_int, c_int]),
+    "pa_tree": (c_int, [ctypes.POINTER(PaKvView), ctypes.POINTER(PaKvScales), c_void_p, c_ll,
+                        c_void_p, c_ll, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int,
+                        c_int, c_int, c_int, c_float, c_void_p, c_size_t, c_void_p]),
+    "logits_adjust": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_ll,
+                              ctypes.POINTER(LogitsRules), c_void_p]),
     "gemm_packed_bytes": (c_size_t, [c_int, c_int, c_int]),
     "gemm_pack_weights": (c_int, [c_int, c_void_p, c_void_p, c_int, c_int, c_void_p]),
     "i8_gemm": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
@@ -249,15 +273,15 @@ _kv_dtypes = None
 
 
 def kv_dtype_of(t) -> int:
-    """llm_dtype of a torch KV pool tensor (fp16, bf16, fp32 or int8)."""
+    """llm_dtype of a torch KV pool tensor (fp16, bf16, fp32, int8 or float8_e4m3fn)."""
     global _kv_dtypes
     if _kv_dtypes is None:
         import torch
         _kv_dtypes = {torch.float16: LLM_F16, torch.bfloat16: LLM_BF16, torch.float32: LLM_F32,
-                      torch.int8: LLM_I8}
+                      torch.int8: LLM_I8, torch.float8_e4m3fn: LLM_E4M3}
     dtype = _kv_dtypes.get(t.dtype)
     if dtype is None:
-        raise TypeError(f"KV pool dtype {t.dtype} is not one of fp16/bf16/fp32/int8")
+        raise TypeError(f"KV pool dtype {t.dtype} is not one of fp16/bf16/fp32/int8/e4m3")
     return dtype
 
 
@@ -352,6 +376,185 @@ def pa_prefill(q, k_pool, v_pool, page_table, *, row, p0, sm_scale=1.0, out=None
     return out
 
 
+def _value_dtype(t, name):
+    import torch
+    dtype = {torch.float32: LLM_F32, torch.float16: LLM_F16, torch.bfloat16: LLM_BF16}.get(t.dtype)
+    if dtype is None:
+        raise TypeError(f"{name} must be fp32, fp16 or bf16, not {t.dtype}")
+    return dtype
+
+
+def _expect(device, **tensors):
+    """Every tensor given: on `device`, of the type and shape that its name is paired with,
+    contiguous (shape None: any)."""
+    for name, (t, dtype, shape) in tensors.items():
+        if t is None:
+            continue
+        if t.device != device:
+            raise ValueError(f"{name} is on {t.device}, not on {device}")
+        if t.dtype != dtype:
+            raise TypeError(f"{name} must be {dtype}, not {t.dtype}")
+        if shape is not None and tuple(t.shape) != shape:
+            raise ValueError(f"{name} must have the shape {shape}, not {tuple(t.shape)}")
+        if not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous")
+
+
+def _on_current(device):
+    import torch
+    if device.type != "cuda" or device.index != torch.cuda.current_device():
+        raise ValueError(f"tensors on {device}: they have to be on the current device")
+
+
+def _token_rows(t, name):
+    """Elements from token to token of [B][N][H][D] (a view of wider tokens, or contiguous)."""
+    B, N, H, D = t.shape
+    step = t.stride(1) if N > 1 else t.stride(0) if B > 1 else H * D
+    if (t.stride(3) != 1 and D > 1) or (t.stride(2) != D and H > 1) or \
+            (B > 1 and N > 1 and t.stride(0) != N * step) or step < H * D:
+        raise ValueError(f"{name} must be [B][N][H][D] with one step between tokens and whole heads in them")
+    return step
+
+
+def kv_scales(k_pool, k_scale, v_scale) -> PaKvScales:
+    """Scales fp32 [num_pages][page_size] of quantised pools [num_pages][page_size][D]; pages
+    of scales may be strided (both the same)."""
+    import torch
+    for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+        if t.dtype != torch.float32:
+            raise TypeError(f"{name} must be fp32, not {t.dtype}")
+        if t.device != k_pool.device:
+            raise ValueError(f"{name} is on {t.device}, not on {k_pool.device}")
+        if t.shape != k_pool.shape[:2] or (t.stride(1) != 1 and t.shape[1] > 1):
+            raise ValueError(f"{name} must be [num_pages][page_size] with contiguous pages")
+    if k_scale.stride(0) != v_scale.stride(0):
+        raise ValueError("k_scale and v_scale must share one page stride")
+    return PaKvScales(k_scale.data_ptr(), v_scale.data_ptr(), k_scale.stride(0))
+
+
+def _paged(k_pool, v_pool, page_table):
+    import torch
+    _on_current(k_pool.device)
+    if v_pool.device != k_pool.device or v_pool.shape != k_pool.shape:
+        raise ValueError("k_pool and v_pool must be of one device and shape")
+    if page_table.dim() != 3:
+        raise ValueError("page_table must be [num_beams][num_heads][max_tiles]")
+    _expect(k_pool.device, page_table=(page_table, torch.int32, None))
+    return kv_view(k_pool, v_pool, page_table)
+
+
+def _quant_call(entry, k, v, k_pool, v_pool, page_table, k_scale, v_scale, starts, lens, beam_ids, stream):
+    import torch
+    view = _paged(k_pool, v_pool, page_table)
+    B, N, H, D = k.shape
+    if v.shape != k.shape or v.dtype != k.dtype or H != page_table.shape[1] or D != k_pool.shape[2]:
+        raise ValueError("k and v must be [B][N][num_heads][head_dim] of one type, as the pages are")
+    step = _token_rows(k, "k")
+    if _token_rows(v, "v") != step:
+        raise ValueError("k and v must have one step between tokens")
+    dev = k_pool.device
+    if k.device != dev or v.device != dev:
+        raise ValueError(f"k and v have to be on {dev}, as the pages are")
+    _expect(dev, starts=(starts, torch.int32, (B,)), lens=(lens, torch.int32, (B,)),
+            beam_ids=(beam_ids, torch.int32, (B,)))
+    if beam_ids is None and B > page_table.shape[0]:
+        raise ValueError("more rows than page_table has beams")
+    scales = kv_scales(k_pool, k_scale, v_scale)
+    check(entry(ctypes.byref(view), ctypes.byref(scales), k.data_ptr(), v.data_ptr(),
+                _value_dtype(k, "k"), step, _at(beam_ids), starts.data_ptr(), _at(lens), B, N,
+                _stream(stream)))
+
+
+def kv_quant_write(k, v, k_pool, v_pool, page_table, k_scale, v_scale, *, starts, lens=None,
+                   beam_ids=None, stream=None):
+    """Quantise K and V of new tokens into their pages: k, v [B][N][H][D] (fp32, fp16 or bf16;
+    views of wider tokens, such as a fused projection's, are taken as they are), row b's token j
+    at position starts[b] + j for j < lens[b].  Pools int8 or float8_e4m3fn [num_pages][ts][D],
+    scales fp32 [num_pages][ts]; both are written in place."""
+    _quant_call(load().kv_quant_write, k, v, k_pool, v_pool, page_table, k_scale, v_scale, starts, lens,
+                beam_ids, stream)
+
+
+def kv_quant_read(k_pool, v_pool, page_table, k_scale, v_scale, *, starts, N=None, lens=None,
+                  beam_ids=None, dtype=None, out=None, stream=None):
+    """Read N tokens a row back from starts[b] on: (k, v) [B][N][H][D] of dtype (default fp32).
+    Tokens past lens[b] are left as they are in out = (k, v), 0 without it."""
+    import torch
+    if stream is not None:  # (what is allocated here belongs to that stream)
+        with torch.cuda.stream(stream):
+            return kv_quant_read(k_pool, v_pool, page_table, k_scale, v_scale, starts=starts, N=N,
+                                 lens=lens, beam_ids=beam_ids, dtype=dtype, out=out)
+    if out is None:
+        shape = (starts.shape[0], N, page_table.shape[1], k_pool.shape[2])
+        make = torch.empty if lens is None else torch.zeros
+        out = tuple(make(shape, dtype=dtype or torch.float32, device=k_pool.device) for _ in "kv")
+    _quant_call(load().kv_quant_read, *out, k_pool, v_pool, page_table, k_scale, v_scale, starts, lens,
+                beam_ids, None)
+    return out
+
+
+def tree_mask(parents):
+    """Mask words int32 [B][N][ceil(N / 32)] of drafted trees: parents [B][N] (or [N]), the place
+    of each token's parent among those ahead of it, -1: the committed context.  A token sees itself and
+    its ancestors."""
+    import torch
+    par = torch.as_tensor(parents).cpu()
+    one = par.dim() == 1
+    par = par.reshape(1, -1) if one else par
+    B, N = par.shape
+    if N and (bool((par >= torch.arange(N)).any()) or bool((par < -1).any())):
+        raise ValueError("a token's parent must be -1 or ahead of it")
+    seen = torch.zeros((B, N, (N + 31) // 32 * 32), dtype=torch.int64)
+    rows = torch.arange(B)
+    for j in range(N):
+        at = par[:, j].long()
+        seen[:, j] = seen[rows, at.clamp(min=0)] * (at >= 0)[:, None]
+        seen[:, j, j] = 1
+    words = (seen.view(B, N, (N + 31) // 32, 32) << torch.arange(32)).sum(-1)
+    words = torch.where(words >= 1 << 31, words - (1 << 32), words).to(torch.int32)
+    return words[0] if one else words
+
+
+def pa_tree(q, k_pool, v_pool, page_table, *, T, context_lens=None, tree_mask=None, tree_lens=None,
+            beam_ids=None, scales=None, sm_scale=1.0, out=None, stream=None):
+    """Attention of drafted tokens over a paged cache: q [B][N][H][D] (fp32, fp16 or bf16; views
+    of wider tokens are taken as they are), whose K and V are in the pages at context_lens[b] + j (T + j
+    without it).  H is a multiple of page_table's heads.  tree_mask int32 words
+    [B][N][ceil(N / 32)], bit j of token i: i sees drafted token j (None: 0 .. i); tree_lens [B]:
+    drafted tokens of each row.  scales = (k_scale, v_scale) of quantised pools.  T bounds the
+    committed tokens.  Returns out [B][N][H][D] of q's type; rows past tree_lens[b] are
+    left as they are in `out`, 0 without it."""
+    import torch
+    if stream is not None:
+        with torch.cuda.stream(stream):
+            return pa_tree(q, k_pool, v_pool, page_table, T=T, context_lens=context_lens,
+                           tree_mask=tree_mask, tree_lens=tree_lens, beam_ids=beam_ids, scales=scales,
+                           sm_scale=sm_scale, out=out)
+    lib = load()
+    view = _paged(k_pool, v_pool, page_table)
+    dev = k_pool.device
+    B, N, H, D = q.shape
+    dtype = _value_dtype(q, "q")
+    if q.device != dev:
+        raise ValueError(f"q is on {q.device}, not on {dev}")
+    if out is None:
+        out = (torch.empty if tree_lens is None else torch.zeros)((B, N, H, D), dtype=q.dtype, device=dev)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev:
+        raise ValueError("out must have q's shape, type and device")
+    _expect(dev, context_lens=(context_lens, torch.int32, (B,)), tree_lens=(tree_lens, torch.int32, (B,)),
+            beam_ids=(beam_ids, torch.int32, (B,)),
+            tree_mask=(tree_mask, torch.int32, (B, N, (N + 31) // 32)))
+    if beam_ids is None and B > page_table.shape[0]:
+        raise ValueError("more rows than page_table has beams")
+    sc = None if scales is None else ctypes.byref(kv_scales(k_pool, *scales))
+    need = lib.pa_tree_workspace_bytes(ctypes.byref(view), B, N, H, T)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    check(lib.pa_tree(ctypes.byref(view), sc, q.data_ptr(), _token_rows(q, "q"), out.data_ptr(),
+                      _token_rows(out, "out"), dtype, _at(beam_ids), _at(context_lens), _at(tree_mask),
+                      _at(tree_lens), B, N, H, D, T, sm_scale, _at(ws), need, _stream(None)))
+    return out
+
+
 def pack_weights(W, dtype: int, stream=None):
     """Repack a device [K][N] int8 / fp16 weight into MFMA fragment order."""
     import torch
@@ -433,6 +636,71 @@ def sample_rows(logits, temperature=1.0, top_k=0, top_p=1.0, seed=0, counter=0, 
     out = torch.empty(R, dtype=torch.int32, device=logits.device)
     check(lib.sample_rows(logits.data_ptr(), R, V, temperature, top_k, top_p, seed, counter,
                           out.data_ptr(), _stream(stream)))
+    return out
+
+
+def logits_adjust(logits, *, history=None, history_lens=None, prompt_lens=None, repetition=None,
+                  frequency=None, presence=None, bias_ids=None, bias=None, allowed=None,
+                  allowed_rows=None, out=None, stream=None):
+    """Penalties for repeated tokens, biases and grammar masks on logits [R][V] (fp32, fp16 or
+    bf16; rows may be strided).  Returns `out` (a new tensor of the logits' layout; out=logits: in
+    place).
+
+    history int32 [R][L] token ids ([L]: one for all rows; ids outside the vocabulary are
+    skipped), of which a row has history_lens[r], the first prompt_lens[r] of them its prompt.  With c
+    the times a token is behind the prompt: x / repetition where x > 0, else x * repetition, for
+    tokens in the history; then - frequency * c - presence * (c > 0); fp32 [R] each.  bias_ids int32
+    and bias fp32 [R][n] (or [n]).  allowed int32 words [M][ceil(V / 32)], bit v set: allowed, -inf
+    else; allowed_rows int32 [R] the row's mask (-1: none; None: mask r)."""
+    import torch
+    if stream is not None:
+        with torch.cuda.stream(stream):
+            return logits_adjust(logits, history=history, history_lens=history_lens,
+                                 prompt_lens=prompt_lens, repetition=repetition, frequency=frequency,
+                                 presence=presence, bias_ids=bias_ids, bias=bias, allowed=allowed,
+                                 allowed_rows=allowed_rows, out=out)
+    R, V = logits.shape
+    dev = logits.device
+    _on_current(dev)
+    dtype = _value_dtype(logits, "logits")
+    stride = logits.stride(0) if R > 1 else V
+    if (logits.stride(1) != 1 and V > 1) or stride < V:
+        raise ValueError("logits must be [R][V] with contiguous rows")
+    if out is None:
+        out = torch.empty_strided((R, V), (stride, 1), dtype=logits.dtype, device=dev)
+    elif out.shape != logits.shape or out.dtype != logits.dtype or out.device != dev or \
+            (out.stride(1) != 1 and V > 1) or (R > 1 and out.stride(0) != stride):
+        raise ValueError("out must have the logits' shape, type, strides and device")
+
+    def listed(name, t, kind):  # ([R][n] or [n]) -> entries a row, from row to row
+        if t is None:
+            return 0, 0
+        _expect(dev, **{name: (t, kind, None)})
+        if t.dim() == 1:
+            return t.shape[0], 0
+        if t.dim() != 2 or t.shape[0] != R:
+            raise ValueError(f"{name} must be [{R}][n] or [n]")
+        return t.shape[1], t.shape[1]
+
+    f32, i32 = torch.float32, torch.int32
+    L, step = listed("history", history, i32)
+    n, bias_step = listed("bias_ids", bias_ids, i32)
+    if (bias is None) != (bias_ids is None) or (bias is not None and bias.shape != bias_ids.shape):
+        raise ValueError("bias_ids and bias go together, of one shape")
+    if allowed is not None and (allowed.dim() != 2 or allowed.shape[1] != (V + 31) // 32):
+        raise ValueError(f"allowed must be [masks][{(V + 31) // 32}]")
+    _expect(dev, history_lens=(history_lens, i32, (R,)), prompt_lens=(prompt_lens, i32, (R,)),
+            repetition=(repetition, f32, (R,)), frequency=(frequency, f32, (R,)),
+            presence=(presence, f32, (R,)), bias=(bias, f32, None), allowed=(allowed, i32, None),
+            allowed_rows=(allowed_rows, i32, (R,)))
+    # (empty lists have no address)
+    rules = LogitsRules(_at(history) if L else None, step, L, _at(history_lens), _at(prompt_lens),
+                        *(_at(t) if L or history is None else None
+                          for t in (repetition, frequency, presence)),
+                        _at(bias_ids) if n else None, _at(bias) if n else None, bias_step, n, _at(allowed),
+                        0 if allowed is None else allowed.shape[0], _at(allowed_rows))
+    check(load().logits_adjust(logits.data_ptr(), out.data_ptr(), dtype, R, V, stride,
+                               ctypes.byref(rules), _stream(None)))
     return out
 
 
