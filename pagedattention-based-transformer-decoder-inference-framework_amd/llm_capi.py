@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
@@ -99,18 +100,16 @@ _SIGS = {
     "pa_decode_ex_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
     "pa_prefill": (c_int, [ctypes.POINTER(PaKvView), c_void_p, c_int, c_void_p, c_int, c_int,
                            c_int, c_int, c_float, c_void_p, c_size_t, c_void_p]),
-    "kv_quant_write": (c_int, [ctypes.POINTER(PaKvView), ctypes.POINTER(PaKvScales), c_void_p,
-                               c_void_p, c_int, c_ll, c_void_p, c_void_p, c_void_p, c_int, c_int,
-                               c_void_p]),
-    "kv_quant_read": (c_int, [ctypes.POINTER(PaKvView), ctypes.POINTER(PaKvScales), c_void_p,
-                              c_void_p, c_int, c_ll, c_void_p, c_void_p, c_void_p, c_int, c_int,
-                              c_void_p]),
-    "pa_tree_workspace_bytes": (c_size_t, [ctypes.POINTER(PaKvView), c_int, c_int, c_int, c_int]),
-    "pa_tree": (c_int, [ctypes.POINTER(PaKvView), ctypes.POINTER(PaKvScales), c_void_p, c_ll,
-                        c_void_p, c_ll, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int,
-                        c_int, c_int, c_int, c_float, c_void_p, c_size_t, c_void_p]),
-    "logits_adjust": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_ll,
-                              ctypes.POINTER(LogitsRules), c_void_p]),
+    # (the structures of these as byref() or as packed bytes)
+    "kv_quant_write": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_ll, c_void_p,
+                               c_void_p, c_void_p, c_int, c_int, c_void_p]),
+    "kv_quant_read": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_ll, c_void_p,
+                              c_void_p, c_void_p, c_int, c_int, c_void_p]),
+    "pa_tree_workspace_bytes": (c_size_t, [c_void_p, c_int, c_int, c_int, c_int]),
+    "pa_tree": (c_int, [c_void_p, c_void_p, c_void_p, c_ll, c_void_p, c_ll, c_int, c_void_p,
+                        c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float,
+                        c_void_p, c_size_t, c_void_p]),
+    "logits_adjust": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_ll, c_void_p, c_void_p]),
     "gemm_packed_bytes": (c_size_t, [c_int, c_int, c_int]),
     "gemm_pack_weights": (c_int, [c_int, c_void_p, c_void_p, c_int, c_int, c_void_p]),
     "i8_gemm": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
@@ -376,93 +375,123 @@ def pa_prefill(q, k_pool, v_pool, page_table, *, row, p0, sm_scale=1.0, out=None
     return out
 
 
+# PaKvView, PaKvScales and LogitsRules as bytes (a structure's constructor takes 1.4 us, its
+# packing 0.4: of a short step's 14 us a call on the host these and the checks took 9).
+_PACK_VIEW, _PACK_SCALES = struct.Struct("@PPP7iq").pack, struct.Struct("@PPq").pack
+_PACK_RULES = struct.Struct("@PqiPPPPPPPqiPiP").pack
+
+_value_dtypes = None
+
+
 def _value_dtype(t, name):
-    import torch
-    dtype = {torch.float32: LLM_F32, torch.float16: LLM_F16, torch.bfloat16: LLM_BF16}.get(t.dtype)
+    global _value_dtypes
+    if _value_dtypes is None:
+        import torch
+        _value_dtypes = {torch.float32: LLM_F32, torch.float16: LLM_F16, torch.bfloat16: LLM_BF16}
+    dtype = _value_dtypes.get(t.dtype)
     if dtype is None:
         raise TypeError(f"{name} must be fp32, fp16 or bf16, not {t.dtype}")
     return dtype
 
 
-def _expect(device, **tensors):
-    """Every tensor given: on `device`, of the type and shape that its name is paired with,
-    contiguous (shape None: any)."""
-    for name, (t, dtype, shape) in tensors.items():
-        if t is None:
-            continue
-        if t.device != device:
-            raise ValueError(f"{name} is on {t.device}, not on {device}")
-        if t.dtype != dtype:
-            raise TypeError(f"{name} must be {dtype}, not {t.dtype}")
-        if shape is not None and tuple(t.shape) != shape:
-            raise ValueError(f"{name} must have the shape {shape}, not {tuple(t.shape)}")
-        if not t.is_contiguous():
-            raise ValueError(f"{name} must be contiguous")
+def _array(t, dev, dtype, shape, name):
+    """Address of an array that a call reads: of `dtype` and `shape` (None: any), contiguous, on
+    device number dev.  None stays None."""
+    if t is None:
+        return None
+    if t.get_device() != dev:
+        raise ValueError(f"{name} is on {t.device}, not on the device of the call's other tensors")
+    if t.dtype is not dtype:
+        raise TypeError(f"{name} must be {dtype}, not {t.dtype}")
+    if shape is not None and t.shape != shape:
+        raise ValueError(f"{name} must have the shape {tuple(shape)}, not {tuple(t.shape)}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    return t.data_ptr()
 
 
-def _on_current(device):
+def _device(t):
+    """Number of a tensor's device, which has to be the current one."""
     import torch
-    if device.type != "cuda" or device.index != torch.cuda.current_device():
-        raise ValueError(f"tensors on {device}: they have to be on the current device")
+    dev = t.get_device()
+    if dev < 0 or dev != torch.cuda.current_device():
+        raise ValueError(f"tensors on {t.device}: they have to be on the current device")
+    return dev
 
 
-def _token_rows(t, name):
+def _token_rows(t, shape, name):
     """Elements from token to token of [B][N][H][D] (a view of wider tokens, or contiguous)."""
-    B, N, H, D = t.shape
-    step = t.stride(1) if N > 1 else t.stride(0) if B > 1 else H * D
-    if (t.stride(3) != 1 and D > 1) or (t.stride(2) != D and H > 1) or \
-            (B > 1 and N > 1 and t.stride(0) != N * step) or step < H * D:
+    B, N, H, D = shape
+    outer, step, head, one = t.stride()
+    if N == 1:
+        step = outer if B > 1 else H * D
+    if (one != 1 and D > 1) or (head != D and H > 1) or (B > 1 and N > 1 and outer != N * step) or step < H * D:
         raise ValueError(f"{name} must be [B][N][H][D] with one step between tokens and whole heads in them")
     return step
+
+
+def _paged(k_pool, v_pool, page_table, dev):
+    """The packed view of pools and table, and (beams, heads) of the table."""
+    import torch
+    shape, strides = k_pool.shape, k_pool.stride()
+    if v_pool.get_device() != dev or v_pool.shape != shape:
+        raise ValueError("k_pool and v_pool must be of one device and shape")
+    if page_table.dim() != 3:
+        raise ValueError("page_table must be [num_beams][num_heads][max_tiles]")
+    table = _array(page_table, dev, torch.int32, None, "page_table")
+    beams, heads, tiles = page_table.shape
+    if len(shape) != 3 or strides[1:] != (shape[2], 1) or v_pool.stride() != strides or \
+            v_pool.dtype is not k_pool.dtype:
+        kv_view(k_pool, v_pool, page_table)  # raises, or a dimension of 1 has a step of its own
+    pages, ts, D = shape
+    kind = kv_dtype_of(k_pool)
+    step = 0 if strides[0] == ts * D or pages == 1 else strides[0] * k_pool.element_size()
+    return _PACK_VIEW(k_pool.data_ptr(), v_pool.data_ptr(), table, pages, ts, D, beams, heads, tiles, kind,
+                      step), beams, heads
+
+
+def _scales(k_pool, k_scale, v_scale, dev):
+    import torch
+    shape, strides = k_scale.shape, k_scale.stride()
+    for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+        if t.dtype is not torch.float32:
+            raise TypeError(f"{name} must be fp32, not {t.dtype}")
+        if t.get_device() != dev:
+            raise ValueError(f"{name} is on {t.device}, not on {k_pool.device}")
+    if shape != k_pool.shape[:2] or v_scale.shape != shape or (strides[1] != 1 and shape[1] > 1):
+        raise ValueError("scales must be [num_pages][page_size] with contiguous pages")
+    if v_scale.stride() != strides:
+        raise ValueError("k_scale and v_scale must share one page stride")
+    return _PACK_SCALES(k_scale.data_ptr(), v_scale.data_ptr(), strides[0] if shape[0] > 1 else 0)
 
 
 def kv_scales(k_pool, k_scale, v_scale) -> PaKvScales:
     """Scales fp32 [num_pages][page_size] of quantised pools [num_pages][page_size][D]; pages
     of scales may be strided (both the same)."""
-    import torch
-    for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
-        if t.dtype != torch.float32:
-            raise TypeError(f"{name} must be fp32, not {t.dtype}")
-        if t.device != k_pool.device:
-            raise ValueError(f"{name} is on {t.device}, not on {k_pool.device}")
-        if t.shape != k_pool.shape[:2] or (t.stride(1) != 1 and t.shape[1] > 1):
-            raise ValueError(f"{name} must be [num_pages][page_size] with contiguous pages")
-    if k_scale.stride(0) != v_scale.stride(0):
-        raise ValueError("k_scale and v_scale must share one page stride")
-    return PaKvScales(k_scale.data_ptr(), v_scale.data_ptr(), k_scale.stride(0))
-
-
-def _paged(k_pool, v_pool, page_table):
-    import torch
-    _on_current(k_pool.device)
-    if v_pool.device != k_pool.device or v_pool.shape != k_pool.shape:
-        raise ValueError("k_pool and v_pool must be of one device and shape")
-    if page_table.dim() != 3:
-        raise ValueError("page_table must be [num_beams][num_heads][max_tiles]")
-    _expect(k_pool.device, page_table=(page_table, torch.int32, None))
-    return kv_view(k_pool, v_pool, page_table)
+    return PaKvScales.from_buffer_copy(_scales(k_pool, k_scale, v_scale, k_pool.get_device()))
 
 
 def _quant_call(entry, k, v, k_pool, v_pool, page_table, k_scale, v_scale, starts, lens, beam_ids, stream):
     import torch
-    view = _paged(k_pool, v_pool, page_table)
-    B, N, H, D = k.shape
-    if v.shape != k.shape or v.dtype != k.dtype or H != page_table.shape[1] or D != k_pool.shape[2]:
+    dev = _device(k_pool)
+    view, beams, heads = _paged(k_pool, v_pool, page_table, dev)
+    shape = k.shape
+    B, N, H, D = shape
+    if v.shape != shape or v.dtype is not k.dtype or H != heads or D != k_pool.shape[2]:
         raise ValueError("k and v must be [B][N][num_heads][head_dim] of one type, as the pages are")
-    step = _token_rows(k, "k")
-    if _token_rows(v, "v") != step:
+    step = _token_rows(k, shape, "k")
+    if v.stride() != k.stride() and _token_rows(v, shape, "v") != step:
         raise ValueError("k and v must have one step between tokens")
-    dev = k_pool.device
-    if k.device != dev or v.device != dev:
-        raise ValueError(f"k and v have to be on {dev}, as the pages are")
-    _expect(dev, starts=(starts, torch.int32, (B,)), lens=(lens, torch.int32, (B,)),
-            beam_ids=(beam_ids, torch.int32, (B,)))
-    if beam_ids is None and B > page_table.shape[0]:
+    if k.get_device() != dev or v.get_device() != dev:
+        raise ValueError(f"k and v have to be on {k_pool.device}, as the pages are")
+    if beam_ids is None and B > beams:
         raise ValueError("more rows than page_table has beams")
-    scales = kv_scales(k_pool, k_scale, v_scale)
-    check(entry(ctypes.byref(view), ctypes.byref(scales), k.data_ptr(), v.data_ptr(),
-                _value_dtype(k, "k"), step, _at(beam_ids), starts.data_ptr(), _at(lens), B, N,
-                _stream(stream)))
+    i32 = torch.int32
+    rc = entry(view, _scales(k_pool, k_scale, v_scale, dev), k.data_ptr(), v.data_ptr(), _value_dtype(k, "k"),
+               step, _array(beam_ids, dev, i32, (B,), "beam_ids"), _array(starts, dev, i32, (B,), "starts"),
+               _array(lens, dev, i32, (B,), "lens"), B, N, _stream(stream))
+    if rc:
+        check(rc)
 
 
 def kv_quant_write(k, v, k_pool, v_pool, page_table, k_scale, v_scale, *, starts, lens=None,
@@ -531,27 +560,31 @@ def pa_tree(q, k_pool, v_pool, page_table, *, T, context_lens=None, tree_mask=No
                            tree_mask=tree_mask, tree_lens=tree_lens, beam_ids=beam_ids, scales=scales,
                            sm_scale=sm_scale, out=out)
     lib = load()
-    view = _paged(k_pool, v_pool, page_table)
-    dev = k_pool.device
-    B, N, H, D = q.shape
+    dev = _device(k_pool)
+    view, beams, _ = _paged(k_pool, v_pool, page_table, dev)
+    shape = q.shape
+    B, N, H, D = shape
     dtype = _value_dtype(q, "q")
-    if q.device != dev:
-        raise ValueError(f"q is on {q.device}, not on {dev}")
+    if q.get_device() != dev:
+        raise ValueError(f"q is on {q.device}, not on {k_pool.device}")
     if out is None:
-        out = (torch.empty if tree_lens is None else torch.zeros)((B, N, H, D), dtype=q.dtype, device=dev)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev:
+        out = (torch.empty if tree_lens is None else torch.zeros)(shape, dtype=q.dtype, device=q.device)
+    elif out.shape != shape or out.dtype is not q.dtype or out.get_device() != dev:
         raise ValueError("out must have q's shape, type and device")
-    _expect(dev, context_lens=(context_lens, torch.int32, (B,)), tree_lens=(tree_lens, torch.int32, (B,)),
-            beam_ids=(beam_ids, torch.int32, (B,)),
-            tree_mask=(tree_mask, torch.int32, (B, N, (N + 31) // 32)))
-    if beam_ids is None and B > page_table.shape[0]:
+    if beam_ids is None and B > beams:
         raise ValueError("more rows than page_table has beams")
-    sc = None if scales is None else ctypes.byref(kv_scales(k_pool, *scales))
-    need = lib.pa_tree_workspace_bytes(ctypes.byref(view), B, N, H, T)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    check(lib.pa_tree(ctypes.byref(view), sc, q.data_ptr(), _token_rows(q, "q"), out.data_ptr(),
-                      _token_rows(out, "out"), dtype, _at(beam_ids), _at(context_lens), _at(tree_mask),
-                      _at(tree_lens), B, N, H, D, T, sm_scale, _at(ws), need, _stream(None)))
+    i32 = torch.int32
+    need = lib.pa_tree_workspace_bytes(view, B, N, H, T)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    rc = lib.pa_tree(view, None if scales is None else _scales(k_pool, *scales, dev), q.data_ptr(),
+                     _token_rows(q, shape, "q"), out.data_ptr(), _token_rows(out, shape, "out"), dtype,
+                     _array(beam_ids, dev, i32, (B,), "beam_ids"),
+                     _array(context_lens, dev, i32, (B,), "context_lens"),
+                     _array(tree_mask, dev, i32, (B, N, (N + 31) // 32), "tree_mask"),
+                     _array(tree_lens, dev, i32, (B,), "tree_lens"), B, N, H, D, T, sm_scale, _at(ws), need,
+                     _stream(None))
+    if rc:
+        check(rc)
     return out
 
 
@@ -659,48 +692,54 @@ def logits_adjust(logits, *, history=None, history_lens=None, prompt_lens=None, 
                                  prompt_lens=prompt_lens, repetition=repetition, frequency=frequency,
                                  presence=presence, bias_ids=bias_ids, bias=bias, allowed=allowed,
                                  allowed_rows=allowed_rows, out=out)
-    R, V = logits.shape
-    dev = logits.device
-    _on_current(dev)
+    dev = _device(logits)
+    R, V = shape = logits.shape
     dtype = _value_dtype(logits, "logits")
-    stride = logits.stride(0) if R > 1 else V
-    if (logits.stride(1) != 1 and V > 1) or stride < V:
+    step, one = logits.stride()
+    if R <= 1:
+        step = V
+    if (one != 1 and V > 1) or step < V:
         raise ValueError("logits must be [R][V] with contiguous rows")
     if out is None:
-        out = torch.empty_strided((R, V), (stride, 1), dtype=logits.dtype, device=dev)
-    elif out.shape != logits.shape or out.dtype != logits.dtype or out.device != dev or \
-            (out.stride(1) != 1 and V > 1) or (R > 1 and out.stride(0) != stride):
+        out = torch.empty_strided(shape, (step, 1), dtype=logits.dtype, device=logits.device)
+    elif out.shape != shape or out.dtype is not logits.dtype or out.get_device() != dev or \
+            (out.stride(1) != 1 and V > 1) or (R > 1 and out.stride(0) != step):
         raise ValueError("out must have the logits' shape, type, strides and device")
 
-    def listed(name, t, kind):  # ([R][n] or [n]) -> entries a row, from row to row
-        if t is None:
-            return 0, 0
-        _expect(dev, **{name: (t, kind, None)})
-        if t.dim() == 1:
-            return t.shape[0], 0
-        if t.dim() != 2 or t.shape[0] != R:
+    def entries(t, name):  # of a row in [R][n] or [n], and from row to row
+        if t.dim() == 2 and t.shape[0] == R:
+            return t.shape[1], t.shape[1]
+        if t.dim() != 1:
             raise ValueError(f"{name} must be [{R}][n] or [n]")
-        return t.shape[1], t.shape[1]
+        return t.shape[0], 0
 
     f32, i32 = torch.float32, torch.int32
-    L, step = listed("history", history, i32)
-    n, bias_step = listed("bias_ids", bias_ids, i32)
-    if (bias is None) != (bias_ids is None) or (bias is not None and bias.shape != bias_ids.shape):
-        raise ValueError("bias_ids and bias go together, of one shape")
-    if allowed is not None and (allowed.dim() != 2 or allowed.shape[1] != (V + 31) // 32):
-        raise ValueError(f"allowed must be [masks][{(V + 31) // 32}]")
-    _expect(dev, history_lens=(history_lens, i32, (R,)), prompt_lens=(prompt_lens, i32, (R,)),
-            repetition=(repetition, f32, (R,)), frequency=(frequency, f32, (R,)),
-            presence=(presence, f32, (R,)), bias=(bias, f32, None), allowed=(allowed, i32, None),
-            allowed_rows=(allowed_rows, i32, (R,)))
     # (empty lists have no address)
-    rules = LogitsRules(_at(history) if L else None, step, L, _at(history_lens), _at(prompt_lens),
-                        *(_at(t) if L or history is None else None
-                          for t in (repetition, frequency, presence)),
-                        _at(bias_ids) if n else None, _at(bias) if n else None, bias_step, n, _at(allowed),
-                        0 if allowed is None else allowed.shape[0], _at(allowed_rows))
-    check(load().logits_adjust(logits.data_ptr(), out.data_ptr(), dtype, R, V, stride,
-                               ctypes.byref(rules), _stream(None)))
+    L = history_step = n = bias_step = masks = 0
+    if history is not None:
+        L, history_step = entries(history, "history")
+    past = [_array(history, dev, i32, None, "history"), _array(history_lens, dev, i32, (R,), "history_lens"),
+            _array(prompt_lens, dev, i32, (R,), "prompt_lens"), _array(repetition, dev, f32, (R,), "repetition"),
+            _array(frequency, dev, f32, (R,), "frequency"), _array(presence, dev, f32, (R,), "presence")]
+    if history is not None and not L:
+        past = [None] * 6
+    if bias_ids is not None or bias is not None:
+        if bias_ids is None or bias is None or bias.shape != bias_ids.shape:
+            raise ValueError("bias_ids and bias go together, of one shape")
+        n, bias_step = entries(bias_ids, "bias_ids")
+    ids, values = _array(bias_ids, dev, i32, None, "bias_ids"), _array(bias, dev, f32, None, "bias")
+    if allowed is not None:
+        if allowed.dim() != 2 or allowed.shape[1] != (V + 31) // 32:
+            raise ValueError(f"allowed must be [masks][{(V + 31) // 32}]")
+        masks = allowed.shape[0]
+    given = [x or 0 for x in past + [ids if n else 0, values if n else 0,
+                                     _array(allowed, dev, i32, None, "allowed"),
+                                     _array(allowed_rows, dev, i32, (R,), "allowed_rows")]]
+    rc = load().logits_adjust(logits.data_ptr(), out.data_ptr(), dtype, R, V, step,
+                              _PACK_RULES(given[0], history_step, L, *given[1:8], bias_step, n, given[8], masks,
+                                          given[9]), _stream(None))
+    if rc:
+        check(rc)
     return out
 
 

@@ -121,3 +121,13 @@ def test_tree_mask():
         llm_capi.tree_mask([0])
     with pytest.raises(ValueError):
         llm_capi.tree_mask([-1, -2])
+
+
+def test_packed_structures():
+    """What the calls pack by hand has the structures' own layout."""
+    def same(kind, packed, values):
+        assert bytes(kind(*values)) == packed(*values) and ctypes.sizeof(kind) == len(packed(*values))
+
+    same(llm_capi.PaKvView, llm_capi._PACK_VIEW, (1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 1 << 40))
+    same(llm_capi.PaKvScales, llm_capi._PACK_SCALES, (1, 2, 1 << 40))
+    same(llm_capi.LogitsRules, llm_capi._PACK_RULES, (1, 1 << 40, 3, 4, 5, 6, 7, 8, 9, 10, 1 << 41, 12, 13, 14, 15))
