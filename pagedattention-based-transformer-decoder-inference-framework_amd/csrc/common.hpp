@@ -219,6 +219,13 @@ __device__ __forceinline__ void load_to_lds(const void* src, void* lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(src)
                : "memory", "m0");
 }
+// ... and 4 bytes per lane, lane l's at lds + 4 l.  (Both: lds within the first 64 KiB of LDS.)
+__device__ __forceinline__ void load_to_lds_dword(const void* src, void* lds) {
+  const uint32_t at = __builtin_amdgcn_readfirstlane(
+      (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)lds);
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(at), "v"(src)
+               : "memory", "m0");
+}
 // The wait (for all but the wave's last LEFT loads, and for its LDS reads) is the
 // builtin: the compiler then knows that its own earlier loads are there too and
 // does not wait for them among the next stage's.

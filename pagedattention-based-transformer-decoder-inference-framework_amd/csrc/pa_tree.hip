@@ -9,29 +9,43 @@ namespace {
 
 constexpr int kMergeThreads = 256;
 
-// A row's parts, relative to the largest of their maxima: D / 4 threads a row.
-__global__ __launch_bounds__(kMergeThreads) void pa_tree_merge_kernel(TreeArgs a, int d4_log) {
-  const long long row = (long long)blockIdx.x * (kMergeThreads >> d4_log) + (threadIdx.x >> d4_log);
-  const int d = (threadIdx.x & ((1 << d4_log) - 1)) * 4, D = 4 << d4_log;
-  if (row >= (long long)a.B * a.N * a.H) return;
+// A row's parts, relative to the largest of their maxima.  A workgroup a row: D / 4 threads hold
+// its dims, the others the same of every (1024 / D)th part.
+template <int D>
+__global__ __launch_bounds__(kMergeThreads) void pa_tree_merge_kernel(TreeArgs a) {
+  constexpr int PER = D / 4, WAYS = kMergeThreads / PER;
+  __shared__ f32x4 s_x[WAYS][PER];
+  __shared__ float s_sum[WAYS];
+  const long long row = blockIdx.x;
   const long long token = row / a.H;
   const int h = (int)(row - token * a.H), b = (int)(token / a.N), i = (int)(token - (long long)b * a.N);
   const TreeRow tr = tree_row(a, b);
   if (i >= tr.n) return;
   const int parts = max((tr.L + tr.split_len - 1) / tr.split_len, 1);
+  const int d = threadIdx.x % PER, way = threadIdx.x / PER;
   const float* ml = a.ml + (size_t)row * a.nsplit * 2;
-  const float* acc = a.acc + (size_t)row * a.nsplit * D + d;
+  const f32x4* acc = reinterpret_cast<const f32x4*>(a.acc + (size_t)row * a.nsplit * D) + d;
   float M = kNegSentinel;
-  for (int s = 0; s < parts; ++s) M = fmaxf(M, ml[2 * s]);
+  for (int s = lane_id(); s < parts; s += 64) M = fmaxf(M, ml[2 * s]);
+  M = wave_max(M);
   float sum = 0.f;
   f32x4 x = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < parts; ++s) {
+#pragma unroll 4
+  for (int s = way; s < parts; s += WAYS) {
     const float weight = __builtin_amdgcn_exp2f(ml[2 * s] - M);
     sum = fmaf(ml[2 * s + 1], weight, sum);
-    x += *reinterpret_cast<const f32x4*>(acc + (size_t)s * D) * weight;
+    x += acc[(size_t)s * PER] * weight;
+  }
+  s_x[way][d] = x;
+  if (d == 0) s_sum[way] = sum;
+  __syncthreads();
+  if (way > 0) return;
+  for (int v = 1; v < WAYS; ++v) {
+    x += s_x[v][d];
+    sum += s_sum[v];
   }
   x *= 1.f / (sum + 1e-6f);
-  const size_t at = (size_t)token * a.out_stride + (size_t)h * D + d;
+  const size_t at = (size_t)token * a.out_stride + (size_t)h * D + 4 * d;
   if (a.dtype == LLM_F32) {
     *reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + at) = x;
   } else if (a.dtype == LLM_F16) {
@@ -69,7 +83,7 @@ TreePlan tree_plan(const pa_kv_view& kv, int B, int N, int H, int T) {
 bool tree_sizes(const pa_kv_view& kv, int B, int N, int H, int T) {
   return B > 0 && B <= 65535 && N > 0 && N <= 1024 && H > 0 && T >= 0 && kv.num_heads > 0 &&
          H % kv.num_heads == 0 && H / kv.num_heads <= 64 && kv.max_tiles > 0 && kv.page_size > 0 &&
-         (long long)B * kv.num_heads <= INT32_MAX / 256;
+         (long long)B * kv.num_heads <= INT32_MAX / 256 && (long long)B * N * H <= INT32_MAX / 256;
 }
 
 }  // namespace
@@ -103,7 +117,7 @@ extern "C" int pa_tree(const pa_kv_view* kv, const pa_kv_scales* scales, const v
   if (B == 0 || N == 0) return LLM_OK;
   if (!tree_sizes(*kv, B, N, H, T))
     return fail(LLM_ERR_UNSUPPORTED, "pa_tree: B <= 65535, N <= 1024, H / num_heads <= 64, "
-                                     "B * num_heads < 2^23");
+                                     "B * num_heads and B * N * H below 2^23");
   LLM_REQUIRE(q && out, "pa_tree: q/out NULL");
   const int es = value_size(dtype);
   if (q_stride == 0) q_stride = (long long)H * D;
@@ -158,11 +172,13 @@ extern "C" int pa_tree(const pa_kv_view* kv, const pa_kv_scales* scales, const v
                                             : launch_tree_e4m3(a, D, p.tiles, grid, st);
   LLM_HIP_RET(e);
   if (p.nsplit > 1) {
-    const int d4_log = D == 64 ? 4 : D == 128 ? 5 : 6, per = kMergeThreads >> d4_log;
-    const long long rows = (long long)B * N * H;
-    LLM_REQUIRE((rows + per - 1) / per <= INT32_MAX / 256, "pa_tree: too many rows");
-    hipLaunchKernelGGL(pa_tree_merge_kernel, dim3((unsigned)((rows + per - 1) / per)), dim3(kMergeThreads), 0, st,
-                       a, d4_log);
+    const dim3 rows((unsigned)((long long)B * N * H));
+    if (D == 64)
+      hipLaunchKernelGGL(pa_tree_merge_kernel<64>, rows, dim3(kMergeThreads), 0, st, a);
+    else if (D == 128)
+      hipLaunchKernelGGL(pa_tree_merge_kernel<128>, rows, dim3(kMergeThreads), 0, st, a);
+    else
+      hipLaunchKernelGGL(pa_tree_merge_kernel<256>, rows, dim3(kMergeThreads), 0, st, a);
     LLM_HIP_RET(hipGetLastError());
   }
   return LLM_OK;

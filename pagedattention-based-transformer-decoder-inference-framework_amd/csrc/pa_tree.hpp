@@ -1,9 +1,10 @@
 // Attention of drafted tokens over a paged cache (pa_tree; its contract is in llm_decoder.h).
 //
 // A workgroup takes rows (tokens x heads of the group) of one key/value head and one split of
-// its keys.  Up to 16 rows are one tile, whose blocks of 32 keys its 4 waves take in turn, merged
-// through LDS; more are 4 tiles, a wave each, which read the same keys at about the same
-// time, from one L1.  All operands come from memory straight into registers, one block ahead:
+// its keys.  Up to 16 rows are one tile, whose blocks of 32 keys its 4 waves take in turn, from
+// memory straight into registers one block ahead, and which are merged through LDS.  More are 4
+// tiles, a wave each; a block goes into LDS once for all four, one block ahead (each wave
+// loading it for itself, L1 gave no more than L2: 16 heads x 63 rows of 32768 e4m3 94 us).
 //   S^T[32 keys][16 rows] = K . Q^T       v_mfma_f32_16x16x32, two tiles of 16 keys
 //   O^T[D][16 rows]      += V^T . P^T
 // A lane (g = lane / 16, c = lane % 16) holds the scores of 8 keys (16 u + 4 g + r; u < 2,

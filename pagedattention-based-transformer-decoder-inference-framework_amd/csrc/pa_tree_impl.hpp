@@ -118,9 +118,18 @@ __global__ __launch_bounds__(64 * kTreeWaves, D <= 128 ? 2 : 1) void pa_tree_ker
   constexpr int NV = ND * ES / 4;     // registers of them
   constexpr int NP = 2;               // parts of a probability
   constexpr int RW = kTreeWaves / KW; // row tiles
+  constexpr bool STAGED = KW == 1;    // keys shared by the waves come through LDS
   constexpr bool AHEAD = ROWB < 512;  // a block ahead of the one in work fits the registers
-  __shared__ float s_acc[kTreeWaves][16][D + 4];
-  __shared__ float s_ml[kTreeWaves][16][2];
+  constexpr int CPR = ROWB / 16;      // 16-byte chunks of a key's row
+  constexpr int kStage = 2 * kTreeKeys * ROWB;  // bytes of a block's K and V
+  // Loads into LDS reach its first 64 KiB: as many stages as fit there, with their scales behind them.
+  constexpr int kScales = QUANT ? kTreeWaves * 256 : 0;  // a wave's own 64: of K, of V
+  constexpr int STAGES = 65536 / (kStage + kScales) < 8 ? 65536 / (kStage + kScales) : 8;
+  constexpr int kSums = kTreeWaves * 16 * (D + 4) * 4, kLoads = STAGED ? STAGES * (kStage + kScales) : 0;
+  __shared__ __align__(16) uint8_t s_mem[kLoads > kSums + 512 ? kLoads : kSums + 512];
+  // behind the last block: the waves' sums
+  float(*s_acc)[16][D + 4] = reinterpret_cast<float(*)[16][D + 4]>(s_mem);
+  float(*s_ml)[16][2] = reinterpret_cast<float(*)[16][2]>(s_mem + kSums);
 
   const int lane = lane_id(), g = lane >> 4, c = lane & 15;
   const int w = wave_id_uniform(), kw = w % KW;
@@ -153,14 +162,32 @@ __global__ __launch_bounds__(64 * kTreeWaves, D <= 128 ? 2 : 1) void pa_tree_ker
     u32x4 k[2][NKL];
     uint32_t v[2][4][NV];
     f32x4 ks[2], vs[2];
-    int page[2];
+    uint32_t here;  // bit u: its u-th 16 keys have a page
+  };
+  auto load_scales = [&](Block& x, int u, int page, int slot) {
+    if constexpr (QUANT) {
+      if (a.k_scale) {
+        const size_t s = (size_t)page * a.scale_stride + slot;
+        const float *ks = a.k_scale + s, *vs = a.v_scale + s;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          x.ks[u][r] = ks[4 * g + r];
+          x.vs[u][r] = vs[4 * g + r];
+        }
+      } else {
+        x.ks[u] = x.vs[u] = f32x4{1.f, 1.f, 1.f, 1.f};
+      }
+    }
   };
   auto load = [&](Block& x, int i) {  // this wave's i-th block
+    x.here = 0;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      x.page[u] = __builtin_amdgcn_readlane(pages, (2 * i + u) & 63);
-      const int page = max(x.page[u], 0);  // (what is read of page 0 instead is masked)
+      const int found = __builtin_amdgcn_readlane(pages, (2 * i + u) & 63);
+      x.here |= (found >= 0 ? 1u : 0u) << u;
+      const int page = max(found, 0);  // (what is read of page 0 instead is masked)
       const int slot = __builtin_amdgcn_readlane(slots, (2 * i + u) & 63);
+      load_scales(x, u, page, slot);
       const size_t base = (size_t)page * a.page_stride + (size_t)slot * ROWB;
       const uint8_t *kp = a.k_pool + base, *vp = a.v_pool + base;
 #pragma unroll
@@ -183,18 +210,77 @@ __global__ __launch_bounds__(64 * kTreeWaves, D <= 128 ? 2 : 1) void pa_tree_ker
           }
         }
       }
-      if constexpr (QUANT) {
-        if (a.k_scale) {
-          const size_t s = (size_t)page * a.scale_stride + slot;
-          const float *ks = a.k_scale + s, *vs = a.v_scale + s;
+    }
+  };
+  // Staged: the workgroup's block i into LDS, K's 32 rows and then V's, 1 KiB an instruction and
+  // lane l's 16 bytes at 16 l of it.  The chunks of a row are exchanged by the key's number, so that
+  // 16 keys' chunks of one column lie in 16 different places of a bank's line.
+  auto exchange = [](int key) {
+    return CPR == 4    ? key >> 2 & 3
+           : CPR == 8  ? key >> 1 & 7
+           : CPR == 16 ? (key << 1 | key >> 3) & 15
+                       : key & 15;
+  };
+  auto stage = [&](int i) {
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            x.ks[u][r] = ks[4 * g + r];
-            x.vs[u][r] = vs[4 * g + r];
+    for (int j = 0; j < kStage / 1024 / kTreeWaves; ++j) {
+      const int at = j * kTreeWaves + w;               // of the instructions
+      const int row = at * (1024 / ROWB) % kTreeKeys;  // its first
+      const int u = row >> 4;
+      const int page = max(__builtin_amdgcn_readlane(pages, (2 * i + u) & 63), 0);
+      const int slot = __builtin_amdgcn_readlane(slots, (2 * i + u) & 63);
+      const uint8_t* pool = at < kStage / 2048 ? a.k_pool : a.v_pool;
+      const int key = (row & 15) + lane / CPR;
+      load_to_lds(pool + (size_t)page * a.page_stride + (size_t)slot * ROWB +
+                      (uint32_t)(key * ROWB + 16 * (lane % CPR ^ exchange(key))),
+                  s_mem + i % STAGES * kStage + at * 1024);
+    }
+    if constexpr (QUANT) {  // lane l: of key l % 32
+      const int p0 = __builtin_amdgcn_readlane(pages, (2 * i) & 63), p1 = __builtin_amdgcn_readlane(pages, (2 * i + 1) & 63);
+      const int s0 = __builtin_amdgcn_readlane(slots, (2 * i) & 63), s1 = __builtin_amdgcn_readlane(slots, (2 * i + 1) & 63);
+      const int u = lane >> 4 & 1;
+      // (without scales anything, so that a stage has the same number of loads)
+      const float* src = reinterpret_cast<const float*>(a.k_pool);
+      if (a.k_scale)
+        src = (lane < 32 ? a.k_scale : a.v_scale) + (size_t)max(u ? p1 : p0, 0) * a.scale_stride + (u ? s1 : s0) + c;
+      load_to_lds_dword(src, s_mem + STAGES * kStage + i % STAGES * kScales + w * 256);
+    }
+  };
+  auto fetch = [&](Block& x, int i) {  // K and V of staged block i
+    const uint8_t* k = s_mem + i % STAGES * kStage;
+    const uint8_t* v = k + kStage / 2;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+#pragma unroll
+      for (int l = 0; l < NKL; ++l)
+        x.k[u][l] = *reinterpret_cast<const u32x4*>(k + (16 * u + c) * ROWB + 16 * ((4 * l + g) ^ exchange(c)));
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int key = 4 * g + r;
+        const uint8_t* row = v + (16 * u + key) * ROWB;
+        if constexpr (NV < 4) {
+          const uint8_t* at = row + 16 * (c * NV / 4 ^ exchange(key)) + c * NV % 4 * 4;
+          if constexpr (NV == 1) {
+            x.v[u][r][0] = *reinterpret_cast<const uint32_t*>(at);
+          } else {
+            const u32x2 y = *reinterpret_cast<const u32x2*>(at);
+            x.v[u][r][0] = y[0], x.v[u][r][1] = y[1];
           }
         } else {
-          x.ks[u] = x.vs[u] = f32x4{1.f, 1.f, 1.f, 1.f};
+#pragma unroll
+          for (int o = 0; o < NV; o += 4) {
+            const u32x4 y = *reinterpret_cast<const u32x4*>(row + 16 * ((c * NV + o) / 4 ^ exchange(key)));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x.v[u][r][o + e] = y[e];
+          }
         }
+      }
+      if constexpr (QUANT) {
+        const float* s = reinterpret_cast<const float*>(s_mem + STAGES * kStage + i % STAGES * kScales + w * 256) +
+                         16 * u + 4 * g;
+        const f32x4 one = {1.f, 1.f, 1.f, 1.f};
+        x.ks[u] = a.k_scale ? *reinterpret_cast<const f32x4*>(s) : one;
+        x.vs[u] = a.k_scale ? *reinterpret_cast<const f32x4*>(s + 32) : one;
       }
     }
   };
@@ -258,7 +344,8 @@ __global__ __launch_bounds__(64 * kTreeWaves, D <= 128 ? 2 : 1) void pa_tree_ker
   f32x4 o[ND];
   // what p is relative to, the maximum (m <= top <= m + kGrow), the sum
   float m = kNegSentinel, top = kNegSentinel, l = 0.f;
-  float unit = 0x1p-100f;  // of the values' scales: a power of two, at least the largest met
+  // of the values' scales: a power of two, at least the largest met; what a probability is multiplied by
+  float unit = 0x1p-100f, per_unit = QUANT ? 0x1p100f * Hf::kP : Hf::kP;
 #pragma unroll
   for (int dd = 0; dd < ND; ++dd) o[dd] = f32x4{0.f, 0.f, 0.f, 0.f};
 
@@ -278,10 +365,10 @@ __global__ __launch_bounds__(64 * kTreeWaves, D <= 128 ? 2 : 1) void pa_tree_ker
     return sh ? w0 >> sh | w1 << (32 - sh) : w0;
   };
   // ... and those of them that anyone may: with a page, ahead of the row's end.
-  auto present_of = [&](const int (&page)[2], int key0) -> uint32_t {
+  auto present_of = [&](uint32_t here, int key0) -> uint32_t {
     uint32_t present = 0xffffffffu;
-    if (page[0] < 0) present &= 0xffff0000u;
-    if (page[1] < 0) present &= 0x0000ffffu;
+    if (!(here & 1u)) present &= 0xffff0000u;
+    if (!(here & 2u)) present &= 0x0000ffffu;
     if (tr.L - key0 < 32) present &= (1u << (tr.L - key0)) - 1u;
     return present;
   };
@@ -289,10 +376,10 @@ __global__ __launch_bounds__(64 * kTreeWaves, D <= 128 ? 2 : 1) void pa_tree_ker
 
   auto attend = [&](Block& x, int i) {
     const int key0 = lo + (i * KW + kw) * kTreeKeys;
-    const bool special = key0 + kTreeKeys > tr.C || x.page[0] < 0 || x.page[1] < 0;
+    const bool special = key0 + kTreeKeys > tr.C || x.here != 3u;
     uint32_t present = 0xffffffffu;
     if (special) {
-      present = present_of(x.page, key0);
+      present = present_of(x.here, key0);
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -369,12 +456,12 @@ __global__ __launch_bounds__(64 * kTreeWaves, D <= 128 ? 2 : 1) void pa_tree_ker
         int e = 0;
         (void)frexpf(rows_max(most), &e);
         const float next = ldexpf(1.f, min(e, 126)), down = unit / next;
+        per_unit = Hf::kP / next;
 #pragma unroll
         for (int dd = 0; dd < ND; ++dd) o[dd] *= down;
         unit = next;
       }
     }
-    const float per_unit = QUANT ? Hf::kP / unit : Hf::kP;
     f32x4 s[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
@@ -391,8 +478,16 @@ __global__ __launch_bounds__(64 * kTreeWaves, D <= 128 ? 2 : 1) void pa_tree_ker
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (!(seen >> (16 * u + 4 * g + r) & 1u)) s[u][r] = -INFINITY;
+        for (int r = 0; r < 4; ++r) {
+          const bool see = seen >> (16 * u + 4 * g + r) & 1u;
+          if (!see) s[u][r] = -INFINITY;
+          if constexpr (QUANT)  // (the scale of what is not seen may be NaN)
+            if (!see) x.vs[u][r] = 0.f;
+        }
+    }
+    if constexpr (QUANT) {
+      x.vs[0] *= per_unit;
+      x.vs[1] *= per_unit;
     }
     float most = -INFINITY;
 #pragma unroll
@@ -420,8 +515,7 @@ __global__ __launch_bounds__(64 * kTreeWaves, D <= 128 ? 2 : 1) void pa_tree_ker
           p[e] = __builtin_amdgcn_exp2f(fmaf(s[u][r], qf, -m));
           l += p[e];
           if constexpr (QUANT) {
-            p[e] *= x.vs[u][r] * per_unit;
-            if (special && !(seen >> (16 * u + 4 * g + r) & 1u)) p[e] = 0.f;  // (the scale may be NaN)
+            p[e] *= x.vs[u][r];
           } else {
             p[e] *= per_unit;
           }
@@ -437,11 +531,40 @@ __global__ __launch_bounds__(64 * kTreeWaves, D <= 128 ? 2 : 1) void pa_tree_ker
       for (int i = 0; i < NP; ++i) o[dd] = Hf::dot(vf[dd], ph[i], o[dd]);
   };
 
-  const int mine = rows > 0 && blocks > kw ? (blocks - kw + KW - 1) / KW : 0;
+  // (staged, waves without rows take their part in the loads)
+  const int mine = (STAGED || rows > 0) && blocks > kw ? (blocks - kw + KW - 1) / KW : 0;
   if (mine > 0) {
     look_up(0);
     Block x;
-    if constexpr (AHEAD) {
+    if constexpr (STAGED) {
+      constexpr int LOADS = kStage / 1024 / kTreeWaves + (QUANT ? 1 : 0);  // of a wave and stage
+      uint64_t there = 0, before = 0;  // bit 2 j + u: block j of the 32 looked up last has half u
+      auto start = [&](int i) {
+        if ((i & 31) == 0) {
+          if (i) look_up(i);
+          before = there;
+          there = __ballot(pages >= 0);
+        }
+        stage(i);
+      };
+      const int ahead = min(STAGES - 1, mine);
+      for (int i = 0; i < ahead; ++i) start(i);
+      for (int i = 0; i < mine; ++i) {
+        if (i + STAGES - 1 <= mine)
+          wait_lds_loads<LOADS*(STAGES - 2)>();
+        else
+          wait_lds_loads();
+        barrier_only();  // block i has landed, block i - 1 is read out
+        const int last = min(i + STAGES - 1, mine - 1);
+        if (i + STAGES - 1 < mine) start(last);
+        if (rows > 0) {
+          x.here = (uint32_t)((last >> 5 == i >> 5 ? there : before) >> (2 * (i & 31))) & 3u;
+          fetch(x, i);
+          attend(x, i);
+        }
+      }
+      __syncthreads();  // the sums take the blocks' place
+    } else if constexpr (AHEAD) {
       Block y;
       load(x, 0);
       for (int i = 0; i < mine; i += 2) {
@@ -463,14 +586,14 @@ __global__ __launch_bounds__(64 * kTreeWaves, D <= 128 ? 2 : 1) void pa_tree_ker
     }
   }
   if constexpr (KVT != LLM_I8)
-    if (__any(unusable)) {
+    if (rows > 0 && __any(unusable)) {
       // The rows that see them get what the products left out: sums of ones count them.
       for (int i = max((tr.C - lo) / (KW * kTreeKeys) - 1, 0); i < mine; ++i) {
         const int key0 = lo + (i * KW + kw) * kTreeKeys;
         if (key0 + kTreeKeys <= tr.C) continue;
         look_up(i);
         const int page[2] = {__builtin_amdgcn_readlane(pages, 0), __builtin_amdgcn_readlane(pages, 1)};
-        const uint32_t present = present_of(page, key0);
+        const uint32_t present = present_of((page[0] >= 0 ? 1u : 0u) | (page[1] >= 0 ? 2u : 0u), key0);
         const uint32_t seen = present & visible(tok, key0);
         u32x4 one;
 #pragma unroll
