@@ -64,10 +64,10 @@ struct TreePlan {
 
 // Splits: as many as bring the launch to about 1024 workgroups, none below 256 keys (the 4
 // waves' two blocks each).
-TreePlan tree_plan(const pa_kv_view& kv, int B, int N, int H, int T) {
+TreePlan tree_plan(const pa_kv_view& kv, int dtype, int B, int N, int H, int T) {
   TreePlan p;
   const int rows = N * (H / kv.num_heads);
-  p.tiles = rows <= 16 ? 1 : kTreeWaves;
+  p.tiles = tree_tiles(kv.head_dim, tree_parts(kv.kv_dtype, dtype), rows);
   p.row_groups = (rows + 16 * p.tiles - 1) / (16 * p.tiles);
   const long long room = (long long)kv.max_tiles * kv.page_size;
   const long long keys = std::max(1LL, std::min((long long)T + N, room));
@@ -93,8 +93,12 @@ using namespace llm;
 
 extern "C" size_t pa_tree_workspace_bytes(const pa_kv_view* kv, int B, int N, int H, int T) {
   if (!kv || !tree_sizes(*kv, B, N, H, T)) return 0;
-  const TreePlan p = tree_plan(*kv, B, N, H, T);
-  return p.nsplit == 1 ? 0 : (size_t)B * N * H * p.nsplit * (kv->head_dim + 2) * sizeof(float);
+  size_t most = 0;  // over the types of q
+  for (int dtype : {LLM_F32, LLM_F16, LLM_BF16}) {
+    const TreePlan p = tree_plan(*kv, dtype, B, N, H, T);
+    if (p.nsplit > 1) most = std::max(most, (size_t)B * N * H * p.nsplit * (kv->head_dim + 2) * sizeof(float));
+  }
+  return most;
 }
 
 extern "C" int pa_tree(const pa_kv_view* kv, const pa_kv_scales* scales, const void* q, long long q_stride,
@@ -125,7 +129,7 @@ extern "C" int pa_tree(const pa_kv_view* kv, const pa_kv_scales* scales, const v
   LLM_REQUIRE(q_stride >= (long long)H * D && out_stride >= (long long)H * D && q_stride * es % 16 == 0 &&
                   out_stride * es % 16 == 0 && aligned16(q) && aligned16(out),
               "pa_tree: rows of q and out must be 16-byte aligned, strides 0 or >= H * D");
-  const TreePlan p = tree_plan(*kv, B, N, H, T);
+  const TreePlan p = tree_plan(*kv, dtype, B, N, H, T);
   LLM_REQUIRE(p.nsplit == 1 || (workspace && aligned16(workspace) &&
                                 workspace_bytes >= pa_tree_workspace_bytes(kv, B, N, H, T)),
               "pa_tree: workspace NULL, not 16-byte aligned or below pa_tree_workspace_bytes");

@@ -1,10 +1,12 @@
 // Attention of drafted tokens over a paged cache (pa_tree; its contract is in llm_decoder.h).
 //
-// A workgroup takes rows (tokens x heads of the group) of one key/value head and one split of
-// its keys.  Up to 16 rows are one tile, whose blocks of 32 keys its 4 waves take in turn, from
-// memory straight into registers one block ahead, and which are merged through LDS.  More are 4
-// tiles, a wave each; a block goes into LDS once for all four, one block ahead (each wave
-// loading it for itself, L1 gave no more than L2: 16 heads x 63 rows of 32768 e4m3 94 us).
+// A workgroup of 4 waves takes rows (tokens x heads of the group) of one key/value head and one
+// split of its keys, in tiles of 16 rows and blocks of 32 keys.  One tile: the waves take its blocks
+// in turn, from memory straight into registers one block ahead.  Up to 4 tiles: two waves of two
+// tiles each take one block, two the next; up to 8: four waves, two tiles each, take the same
+// block.  Keys that waves share go into LDS once, stages ahead (16 heads x 63 rows of 32768 e4m3
+// tokens: each wave loading them for itself 94 us, L1 gave no more than L2).  Two tiles a wave share
+// the conversions and exchanges of the keys.  Waves with the same rows are merged through LDS.
 //   S^T[32 keys][16 rows] = K . Q^T       v_mfma_f32_16x16x32, two tiles of 16 keys
 //   O^T[D][16 rows]      += V^T . P^T
 // A lane (g = lane / 16, c = lane % 16) holds the scores of 8 keys (16 u + 4 g + r; u < 2,
@@ -71,6 +73,17 @@ __device__ __forceinline__ TreeRow tree_row(const TreeArgs& a, int b) {
   const int even = ((r.L + a.nsplit - 1) / a.nsplit + kTreeStep - 1) / kTreeStep * kTreeStep;
   r.split_len = max(a.split_keys, even);
   return r;
+}
+
+// Parts of a query: the products' type is bf16 over bf16 pools, else fp16.
+constexpr int tree_parts(int kvt, int dtype) {
+  return kvt == LLM_BF16 ? (dtype == LLM_F32 ? 3 : dtype == LLM_F16 ? 2 : 1) : dtype == LLM_F32 ? 2 : 1;
+}
+// Row tiles of a wave where a workgroup's keys come through LDS: queries and sums of two fit the
+// registers of two waves a SIMD up to 128 dims of query parts.  And of a workgroup for `rows` rows.
+constexpr int tree_wave_tiles(int D, int parts) { return D * parts <= 128 ? 2 : 1; }
+inline int tree_tiles(int D, int parts, int rows) {
+  return rows <= 16 ? 1 : rows <= 64 ? 4 : 4 * tree_wave_tiles(D, parts);
 }
 
 // pa_tree_*.hip

@@ -106,8 +106,9 @@ __device__ __forceinline__ uint32_t usable(uint32_t w) {
   return kept;
 }
 
-// NQ: parts of a query; KW: waves that share a row tile's keys, the others have tiles of their own.
-template <int KVT, int D, int NQ, int KW>
+// NQ, NP: parts of a query, of a probability; KW: waves that share the keys of the same rows, the others
+// have rows of their own; MT: row tiles of a wave.
+template <int KVT, int D, int NQ, int NP, int KW, int MT>
 __global__ __launch_bounds__(64 * kTreeWaves, D <= 128 ? 2 : 1) void pa_tree_kernel(TreeArgs a) {
   constexpr bool QUANT = Raw<KVT>::QUANT;
   constexpr int ES = Raw<KVT>::ES, ROWB = D * ES;
@@ -116,15 +117,16 @@ __global__ __launch_bounds__(64 * kTreeWaves, D <= 128 ? 2 : 1) void pa_tree_ker
   constexpr int NKL = ROWB / 64;      // 16-byte loads of a key tile
   constexpr int ND = D / 16;          // tiles of the output, dims of a lane's keys
   constexpr int NV = ND * ES / 4;     // registers of them
-  constexpr int NP = 2;               // parts of a probability
-  constexpr int RW = kTreeWaves / KW; // row tiles
-  constexpr bool STAGED = KW == 1;    // keys shared by the waves come through LDS
+  constexpr int RW = kTreeWaves / KW; // waves with rows of their own
+  constexpr bool STAGED = KW < kTreeWaves;  // keys shared by waves come through LDS
   constexpr bool AHEAD = ROWB < 512;  // a block ahead of the one in work fits the registers
   constexpr int CPR = ROWB / 16;      // 16-byte chunks of a key's row
-  constexpr int kStage = 2 * kTreeKeys * ROWB;  // bytes of a block's K and V
+  constexpr int kBlock = 2 * kTreeKeys * ROWB, kStage = KW * kBlock;  // bytes of a block's K and V, of KW blocks'
+  static_assert(STAGED || MT == 1, "what is loaded ahead leaves no room for more tiles");
   // Loads into LDS reach its first 64 KiB: as many stages as fit there, with their scales behind them.
   constexpr int kScales = QUANT ? kTreeWaves * 256 : 0;  // a wave's own 64: of K, of V
-  constexpr int STAGES = 65536 / (kStage + kScales) < 8 ? 65536 / (kStage + kScales) : 8;
+  constexpr int STAGES = !STAGED ? 1 : 65536 / (kStage + kScales) < 8 ? 65536 / (kStage + kScales) : 8;
+  static_assert(!STAGED || STAGES >= 2, "a stage ahead");
   constexpr int kSums = kTreeWaves * 16 * (D + 4) * 4, kLoads = STAGED ? STAGES * (kStage + kScales) : 0;
   __shared__ __align__(16) uint8_t s_mem[kLoads > kSums + 512 ? kLoads : kSums + 512];
   // behind the last block: the waves' sums
@@ -132,12 +134,14 @@ __global__ __launch_bounds__(64 * kTreeWaves, D <= 128 ? 2 : 1) void pa_tree_ker
   float(*s_ml)[16][2] = reinterpret_cast<float(*)[16][2]>(s_mem + kSums);
 
   const int lane = lane_id(), g = lane >> 4, c = lane & 15;
-  const int w = wave_id_uniform(), kw = w % KW;
+  const int w = wave_id_uniform(), kw = w % KW, rw = w / KW;
   const int pair = blockIdx.x, b = pair / a.kv_heads, kvh = pair - b * a.kv_heads;
   const int split = blockIdx.y;
   const TreeRow tr = tree_row(a, b);
-  const int first = blockIdx.z * 16 * RW, row0 = first + w / KW * 16;  // of the workgroup, the wave
-  const int all_rows = tr.n * a.G, rows = all_rows - row0;
+  const int first = blockIdx.z * 16 * RW * MT, all_rows = tr.n * a.G;
+  // the wave's tiles: rows row_of(t) .. + 15, of which the row has rows_of(t)
+  auto row_of = [&](int t) { return first + 16 * (rw + RW * t); };
+  auto rows_of = [&](int t) { return all_rows - row_of(t); };
   const int lo = split * tr.split_len;
   if (first >= all_rows || (split > 0 && lo >= tr.L)) return;
   const int hi = min(lo + tr.split_len, tr.L);
@@ -146,15 +150,23 @@ __global__ __launch_bounds__(64 * kTreeWaves, D <= 128 ? 2 : 1) void pa_tree_ker
   const int32_t* pt = a.table + ((size_t)(has_beam ? beam : 0) * a.kv_heads + kvh) * a.max_tiles;
   const int blocks = (hi - lo + kTreeKeys - 1) / kTreeKeys;
 
-  // Lane i: the page of 16 keys, half i % 2 of this wave's block number from + i / 2 (-1: none),
-  // and where in it they begin.
+  // Lane i: the page of 16 keys (-1: none) and where in it they begin, of the 64 halves from block
+  // `from` on: this wave's own blocks, or, staged, all.
+  constexpr int LOOKED = STAGED ? 32 / KW : 32;  // turns of a look-up
   int pages, slots;
-  auto look_up = [&](int from) {
-    const int key = lo + ((from + (lane >> 1)) * KW + kw) * kTreeKeys + 16 * (lane & 1);
+  auto look_up = [&](int key) {
     const int tile = key / a.page_size;
     slots = key - tile * a.page_size;
     const int p = has_beam && key < hi ? pt[tile] : -1;
     pages = p >= 0 && p < a.num_pages ? p : -1;
+  };
+  auto look_up_from = [&](int i) {
+    look_up(STAGED ? lo + i * KW * kTreeKeys + 16 * lane
+                   : lo + ((i + (lane >> 1)) * KW + kw) * kTreeKeys + 16 * (lane & 1));
+  };
+  // ... the lane of half u of block `block` of turn i
+  auto half_of = [&](int i, int block, int u) {
+    return STAGED ? (i % LOOKED * KW + block) * 2 + u : (2 * i + u) & 63;
   };
 
   // a block's operands as they are in memory
@@ -183,10 +195,10 @@ __global__ __launch_bounds__(64 * kTreeWaves, D <= 128 ? 2 : 1) void pa_tree_ker
     x.here = 0;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const int found = __builtin_amdgcn_readlane(pages, (2 * i + u) & 63);
+      const int found = __builtin_amdgcn_readlane(pages, half_of(i, 0, u));
       x.here |= (found >= 0 ? 1u : 0u) << u;
       const int page = max(found, 0);  // (what is read of page 0 instead is masked)
-      const int slot = __builtin_amdgcn_readlane(slots, (2 * i + u) & 63);
+      const int slot = __builtin_amdgcn_readlane(slots, half_of(i, 0, u));
       load_scales(x, u, page, slot);
       const size_t base = (size_t)page * a.page_stride + (size_t)slot * ROWB;
       const uint8_t *kp = a.k_pool + base, *vp = a.v_pool + base;
@@ -212,9 +224,9 @@ __global__ __launch_bounds__(64 * kTreeWaves, D <= 128 ? 2 : 1) void pa_tree_ker
       }
     }
   };
-  // Staged: the workgroup's block i into LDS, K's 32 rows and then V's, 1 KiB an instruction and
-  // lane l's 16 bytes at 16 l of it.  The chunks of a row are exchanged by the key's number, so that
-  // 16 keys' chunks of one column lie in 16 different places of a bank's line.
+  // Staged: the KW blocks of turn i into LDS, each K's 32 rows and then V's, 1 KiB an instruction
+  // and lane l's 16 bytes at 16 l of it.  The chunks of a row are exchanged by the key's number, so
+  // that 16 keys' chunks of one column lie in 16 different places of a bank's line.
   auto exchange = [](int key) {
     return CPR == 4    ? key >> 2 & 3
            : CPR == 8  ? key >> 1 & 7
@@ -225,19 +237,21 @@ __global__ __launch_bounds__(64 * kTreeWaves, D <= 128 ? 2 : 1) void pa_tree_ker
 #pragma unroll
     for (int j = 0; j < kStage / 1024 / kTreeWaves; ++j) {
       const int at = j * kTreeWaves + w;               // of the instructions
+      const int block = at / (kBlock / 1024);
       const int row = at * (1024 / ROWB) % kTreeKeys;  // its first
-      const int u = row >> 4;
-      const int page = max(__builtin_amdgcn_readlane(pages, (2 * i + u) & 63), 0);
-      const int slot = __builtin_amdgcn_readlane(slots, (2 * i + u) & 63);
-      const uint8_t* pool = at < kStage / 2048 ? a.k_pool : a.v_pool;
+      const int half = half_of(i, block, row >> 4);
+      const int page = max(__builtin_amdgcn_readlane(pages, half), 0);
+      const int slot = __builtin_amdgcn_readlane(slots, half);
+      const uint8_t* pool = at % (kBlock / 1024) < kBlock / 2048 ? a.k_pool : a.v_pool;
       const int key = (row & 15) + lane / CPR;
       load_to_lds(pool + (size_t)page * a.page_stride + (size_t)slot * ROWB +
                       (uint32_t)(key * ROWB + 16 * (lane % CPR ^ exchange(key))),
                   s_mem + i % STAGES * kStage + at * 1024);
     }
-    if constexpr (QUANT) {  // lane l: of key l % 32
-      const int p0 = __builtin_amdgcn_readlane(pages, (2 * i) & 63), p1 = __builtin_amdgcn_readlane(pages, (2 * i + 1) & 63);
-      const int s0 = __builtin_amdgcn_readlane(slots, (2 * i) & 63), s1 = __builtin_amdgcn_readlane(slots, (2 * i + 1) & 63);
+    if constexpr (QUANT) {  // this wave's block, lane l: of key l % 32
+      const int h0 = half_of(i, kw, 0), h1 = half_of(i, kw, 1);
+      const int p0 = __builtin_amdgcn_readlane(pages, h0), p1 = __builtin_amdgcn_readlane(pages, h1);
+      const int s0 = __builtin_amdgcn_readlane(slots, h0), s1 = __builtin_amdgcn_readlane(slots, h1);
       const int u = lane >> 4 & 1;
       // (without scales anything, so that a stage has the same number of loads)
       const float* src = reinterpret_cast<const float*>(a.k_pool);
@@ -246,9 +260,9 @@ __global__ __launch_bounds__(64 * kTreeWaves, D <= 128 ? 2 : 1) void pa_tree_ker
       load_to_lds_dword(src, s_mem + STAGES * kStage + i % STAGES * kScales + w * 256);
     }
   };
-  auto fetch = [&](Block& x, int i) {  // K and V of staged block i
-    const uint8_t* k = s_mem + i % STAGES * kStage;
-    const uint8_t* v = k + kStage / 2;
+  auto fetch = [&](Block& x, int i) {  // this wave's block of turn i
+    const uint8_t* k = s_mem + i % STAGES * kStage + kw * kBlock;
+    const uint8_t* v = k + kBlock / 2;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
 #pragma unroll
@@ -286,14 +300,17 @@ __global__ __launch_bounds__(64 * kTreeWaves, D <= 128 ? 2 : 1) void pa_tree_ker
   };
 
   // Queries: lane (g, c) holds row c's dims, those of the 16 bytes of K that it loads.
-  u32x4 q[NQ][NK];
-  float qf = fmaxf(fabsf(a.scale2), 1e-37f);  // what its scores are multiplied by, in log2 units: > 0, so
-                                              // that -infinity stays what it is
-  const int tok = (row0 + (c < rows ? c : 0)) / a.G;
-  {
-    const bool ok = c < rows;
-    const int h = kvh * a.G + row0 + (ok ? c : 0) - tok * a.G;
-    const size_t at = ((size_t)b * a.N + (ok ? tok : 0)) * a.q_stride + (size_t)(ok ? h : 0) * D;
+  u32x4 q[MT][NQ][NK];
+  float qf[MT];  // what its scores are multiplied by, in log2 units: > 0, so that -infinity stays what it is
+  int tok[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) {
+    const bool ok = c < rows_of(t);
+    const int row = ok ? row_of(t) + c : 0;  // (no row: the first one's place, as zeros)
+    tok[t] = row / a.G;
+    const int h = kvh * a.G + row - tok[t] * a.G;
+    const size_t at = ((size_t)b * a.N + tok[t]) * a.q_stride + (size_t)h * D;
+    qf[t] = fmaxf(fabsf(a.scale2), 1e-37f);
     float x[NK][8];
     float most = 0.f;
 #pragma unroll
@@ -324,7 +341,7 @@ __global__ __launch_bounds__(64 * kTreeWaves, D <= 128 ? 2 : 1) void pa_tree_ker
       (void)frexpf(rows_max(most), &e);  // most < 2^e
       e = clamp_int(e, -100, 100);
       const float up = ldexpf(1.f, 14 - e);
-      qf = fmaxf(qf * ldexpf(1.f, e - 14), 1e-37f);
+      qf[t] = fmaxf(qf[t] * ldexpf(1.f, e - 14), 1e-37f);
 #pragma unroll
       for (int kk = 0; kk < NK; ++kk)
 #pragma unroll
@@ -337,17 +354,21 @@ __global__ __launch_bounds__(64 * kTreeWaves, D <= 128 ? 2 : 1) void pa_tree_ker
         uint32_t part[NQ];
         split_parts<Hf, NQ>(x[kk][2 * i], x[kk][2 * i + 1], part);
 #pragma unroll
-        for (int p = 0; p < NQ; ++p) q[p][kk][i] = part[p];
+        for (int p = 0; p < NQ; ++p) q[t][p][kk][i] = part[p];
       }
   }
 
-  f32x4 o[ND];
-  // what p is relative to, the maximum (m <= top <= m + kGrow), the sum
-  float m = kNegSentinel, top = kNegSentinel, l = 0.f;
+  f32x4 o[MT][ND];
+  float m[MT], top[MT], l[MT];  // what p is relative to, the maximum (m <= top <= m + kGrow), the sum
   // of the values' scales: a power of two, at least the largest met; what a probability is multiplied by
   float unit = 0x1p-100f, per_unit = QUANT ? 0x1p100f * Hf::kP : Hf::kP;
 #pragma unroll
-  for (int dd = 0; dd < ND; ++dd) o[dd] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int t = 0; t < MT; ++t) {
+    m[t] = top[t] = kNegSentinel;
+    l[t] = 0.f;
+#pragma unroll
+    for (int dd = 0; dd < ND; ++dd) o[t][dd] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
 
   // Keys key0 .. key0 + 31 that a drafted token sees, as far as its mask says.
   auto visible = [&](int token, int key0) -> uint32_t {
@@ -448,100 +469,106 @@ __global__ __launch_bounds__(64 * kTreeWaves, D <= 128 ? 2 : 1) void pa_tree_ker
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float s = fabsf(x.vs[u][r]);
-          if (s < INFINITY) most = fmaxf(most, s);
-        }
+        for (int r = 0; r < 4; ++r) most = fmaxf(most, fabsf(x.vs[u][r]));
       if (__any(most > unit)) {
+        most = 0.f;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (fabsf(x.vs[u][r]) < INFINITY) most = fmaxf(most, fabsf(x.vs[u][r]));
         int e = 0;
-        (void)frexpf(rows_max(most), &e);
+        (void)frexpf(fmaxf(rows_max(most), unit * 0.75f), &e);
         const float next = ldexpf(1.f, min(e, 126)), down = unit / next;
         per_unit = Hf::kP / next;
 #pragma unroll
-        for (int dd = 0; dd < ND; ++dd) o[dd] *= down;
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+          for (int dd = 0; dd < ND; ++dd) o[t][dd] *= down;
         unit = next;
       }
-    }
-    f32x4 s[2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int p = 0; p < NQ; ++p)
-#pragma unroll
-        for (int kk = 0; kk < NK; ++kk) s[u] = Hf::dot(kf[u][kk], q[p][kk], s[u]);
-      if constexpr (QUANT) s[u] *= x.ks[u];
-    }
-    uint32_t seen = present;
-    if (special) {
-      seen &= visible(tok, key0);
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const bool see = seen >> (16 * u + 4 * g + r) & 1u;
-          if (!see) s[u][r] = -INFINITY;
-          if constexpr (QUANT)  // (the scale of what is not seen may be NaN)
-            if (!see) x.vs[u][r] = 0.f;
-        }
-    }
-    if constexpr (QUANT) {
       x.vs[0] *= per_unit;
       x.vs[1] *= per_unit;
     }
-    float most = -INFINITY;
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+    for (int t = 0; t < MT; ++t) {
+      if (t > 0 && rows_of(t) <= 0) break;
+      f32x4 s[2], vs[2];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) most = fmaxf(most, s[u][r]);
-    most = rows_max(most) * qf;
-    top = fmaxf(top, most);
-    if (__any(most > m + Hf::kGrow)) {
-      const float corr = __builtin_amdgcn_exp2f(m - top);
-      l *= corr;
+      for (int u = 0; u < 2; ++u) {
+        s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int dd = 0; dd < ND; ++dd) o[dd] *= corr;
-      m = top;
-    }
-    u32x4 ph[NP];
+        for (int p = 0; p < NQ; ++p)
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        float p[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int r = 2 * hf + e;
-          p[e] = __builtin_amdgcn_exp2f(fmaf(s[u][r], qf, -m));
-          l += p[e];
-          if constexpr (QUANT) {
-            p[e] *= x.vs[u][r];
-          } else {
-            p[e] *= per_unit;
-          }
+          for (int kk = 0; kk < NK; ++kk) s[u] = Hf::dot(kf[u][kk], q[t][p][kk], s[u]);
+        if constexpr (QUANT) {
+          s[u] *= x.ks[u];
+          vs[u] = x.vs[u];
         }
-        uint32_t part[NP];
-        split_parts<Hf, NP>(p[0], p[1], part);
-#pragma unroll
-        for (int i = 0; i < NP; ++i) ph[i][2 * u + hf] = part[i];
       }
+      if (special) {
+        const uint32_t seen = present & visible(tok[t], key0);
 #pragma unroll
-    for (int dd = 0; dd < ND; ++dd)
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int i = 0; i < NP; ++i) o[dd] = Hf::dot(vf[dd], ph[i], o[dd]);
+          for (int r = 0; r < 4; ++r) {
+            const bool see = seen >> (16 * u + 4 * g + r) & 1u;
+            if (!see) s[u][r] = -INFINITY;
+            if constexpr (QUANT)  // (the scale of what is not seen may be NaN)
+              if (!see) vs[u][r] = 0.f;
+          }
+      }
+      float most = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) most = fmaxf(most, s[u][r]);
+      most = rows_max(most) * qf[t];
+      top[t] = fmaxf(top[t], most);
+      if (__any(most > m[t] + Hf::kGrow)) {
+        const float corr = __builtin_amdgcn_exp2f(m[t] - top[t]);
+        l[t] *= corr;
+#pragma unroll
+        for (int dd = 0; dd < ND; ++dd) o[t][dd] *= corr;
+        m[t] = top[t];
+      }
+      u32x4 ph[NP];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          float p[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int r = 2 * hf + e;
+            p[e] = __builtin_amdgcn_exp2f(fmaf(s[u][r], qf[t], -m[t]));
+            l[t] += p[e];
+            p[e] *= QUANT ? vs[u][r] : per_unit;
+          }
+          uint32_t part[NP];
+          split_parts<Hf, NP>(p[0], p[1], part);
+#pragma unroll
+          for (int i = 0; i < NP; ++i) ph[i][2 * u + hf] = part[i];
+        }
+#pragma unroll
+      for (int dd = 0; dd < ND; ++dd)
+#pragma unroll
+        for (int i = 0; i < NP; ++i) o[t][dd] = Hf::dot(vf[dd], ph[i], o[t][dd]);
+    }
   };
 
-  // (staged, waves without rows take their part in the loads)
-  const int mine = (STAGED || rows > 0) && blocks > kw ? (blocks - kw + KW - 1) / KW : 0;
+  // Turns; staged, waves without rows, or without a block in the last one, take their part in the loads.
+  const int mine = STAGED ? (blocks + KW - 1) / KW
+                          : blocks > kw ? (blocks - kw + KW - 1) / KW : 0;
   if (mine > 0) {
-    look_up(0);
+    look_up_from(0);
     Block x;
     if constexpr (STAGED) {
       constexpr int LOADS = kStage / 1024 / kTreeWaves + (QUANT ? 1 : 0);  // of a wave and stage
-      uint64_t there = 0, before = 0;  // bit 2 j + u: block j of the 32 looked up last has half u
+      uint64_t there = 0, before = 0;  // the halves looked up last, and those before, that have a page
       auto start = [&](int i) {
-        if ((i & 31) == 0) {
-          if (i) look_up(i);
+        if (i % LOOKED == 0) {
+          if (i) look_up_from(i);
           before = there;
           there = __ballot(pages >= 0);
         }
@@ -557,8 +584,8 @@ __global__ __launch_bounds__(64 * kTreeWaves, D <= 128 ? 2 : 1) void pa_tree_ker
         barrier_only();  // block i has landed, block i - 1 is read out
         const int last = min(i + STAGES - 1, mine - 1);
         if (i + STAGES - 1 < mine) start(last);
-        if (rows > 0) {
-          x.here = (uint32_t)((last >> 5 == i >> 5 ? there : before) >> (2 * (i & 31))) & 3u;
+        if (rows_of(0) > 0 && i * KW + kw < blocks) {
+          x.here = (uint32_t)((last / LOOKED == i / LOOKED ? there : before) >> half_of(i, kw, 0)) & 3u;
           fetch(x, i);
           attend(x, i);
         }
@@ -572,34 +599,37 @@ __global__ __launch_bounds__(64 * kTreeWaves, D <= 128 ? 2 : 1) void pa_tree_ker
         attend(x, i);
         if (i + 1 >= mine) break;
         if (i + 2 < mine) {
-          if (((i + 2) & 31) == 0) look_up(i + 2);
+          if (((i + 2) & 31) == 0) look_up_from(i + 2);
           load(x, i + 2);
         }
         attend(y, i + 1);
       }
     } else {
       for (int i = 0; i < mine; ++i) {
-        if (i && (i & 31) == 0) look_up(i);
+        if (i && (i & 31) == 0) look_up_from(i);
         load(x, i);
         attend(x, i);
       }
     }
   }
   if constexpr (KVT != LLM_I8)
-    if (rows > 0 && __any(unusable)) {
+    if (__any(unusable)) {
       // The rows that see them get what the products left out: sums of ones count them.
       for (int i = max((tr.C - lo) / (KW * kTreeKeys) - 1, 0); i < mine; ++i) {
         const int key0 = lo + (i * KW + kw) * kTreeKeys;
-        if (key0 + kTreeKeys <= tr.C) continue;
-        look_up(i);
+        if (key0 + kTreeKeys <= tr.C || key0 >= hi) continue;
+        look_up(key0 + 16 * (lane & 1));
         const int page[2] = {__builtin_amdgcn_readlane(pages, 0), __builtin_amdgcn_readlane(pages, 1)};
         const uint32_t present = present_of((page[0] >= 0 ? 1u : 0u) | (page[1] >= 0 ? 2u : 0u), key0);
-        const uint32_t seen = present & visible(tok, key0);
-        u32x4 one;
+        u32x4 one[MT];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t two = seen >> (16 * (e / 2) + 4 * g + 2 * (e % 2));
-          one[e] = (two & 1u ? Hf::kOne : 0u) | (two & 2u ? Hf::kOne << 16 : 0u);
+        for (int t = 0; t < MT; ++t) {
+          const uint32_t seen = present & visible(tok[t], key0);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t two = seen >> (16 * (e / 2) + 4 * g + 2 * (e % 2));
+            one[t][e] = (two & 1u ? Hf::kOne : 0u) | (two & 2u ? Hf::kOne << 16 : 0u);
+          }
         }
 #pragma unroll
         for (int dd = 0; dd < ND; ++dd) {
@@ -621,33 +651,39 @@ __global__ __launch_bounds__(64 * kTreeWaves, D <= 128 ? 2 : 1) void pa_tree_ker
             }
           }
           const f32x4 none = {0.f, 0.f, 0.f, 0.f};
-          const f32x4 up = Hf::dot(plus, one, none), down = Hf::dot(minus, one, none);
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            o[dd][r] += (up[r] > 0.f ? INFINITY : 0.f) - (down[r] > 0.f ? INFINITY : 0.f);
+          for (int t = 0; t < MT; ++t) {
+            const f32x4 up = Hf::dot(plus, one[t], none), down = Hf::dot(minus, one[t], none);
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              o[t][dd][r] += (up[r] > 0.f ? INFINITY : 0.f) - (down[r] > 0.f ? INFINITY : 0.f);
+          }
         }
       }
     }
 
   // The sums of a tile's waves, relative to the largest maximum of the row.
-  const float back = __builtin_amdgcn_exp2f(m - top);
-  const float sum = add(with_lane32(add(with_lane16(l * back))));
+  const int rr = threadIdx.x >> 4, part = threadIdx.x & 15;  // a row, ND of its dims
+#pragma unroll
+  for (int t = 0; t < MT; ++t) {
+  const float back = __builtin_amdgcn_exp2f(m[t] - top[t]);
+  const float sum = add(with_lane32(add(with_lane16(l[t] * back))));
   const float f = back * (QUANT ? unit / Hf::kP : 1.f / Hf::kP);
+  if (t) __syncthreads();  // the tiles before are read
 #pragma unroll
   for (int r = 0; r < 4; ++r)
 #pragma unroll
     for (int dd = 0; dd < ND; dd += 4)
       *reinterpret_cast<f32x4*>(&s_acc[w][c][(4 * g + r) * ND + dd]) =
-          f32x4{o[dd][r] * f, o[dd + 1][r] * f, o[dd + 2][r] * f, o[dd + 3][r] * f};
+          f32x4{o[t][dd][r] * f, o[t][dd + 1][r] * f, o[t][dd + 2][r] * f, o[t][dd + 3][r] * f};
   if (g == 0) {
-    s_ml[w][c][0] = top;
+    s_ml[w][c][0] = top[t];
     s_ml[w][c][1] = sum;
   }
   __syncthreads();
-  const int rr = threadIdx.x >> 4, part = threadIdx.x & 15;  // a row, ND of its dims
 #pragma unroll
   for (int tile = 0; tile < RW; ++tile) {
-    const int row = first + 16 * tile + rr;
+    const int row = first + 16 * (tile + RW * t) + rr;
     if (row >= all_rows) break;
     float M = kNegSentinel;
 #pragma unroll
@@ -685,27 +721,39 @@ __global__ __launch_bounds__(64 * kTreeWaves, D <= 128 ? 2 : 1) void pa_tree_ker
       }
     }
   }
+  }
 }
 
-template <int KVT, int D, int NQ>
+// tiles: row tiles of a workgroup (tree_tiles).
+template <int KVT, int D, int NQ, int NP>
 hipError_t launch_tree_tiles(const TreeArgs& a, int tiles, dim3 grid, hipStream_t st) {
-  hipLaunchKernelGGL((tiles == 1 ? pa_tree_kernel<KVT, D, NQ, kTreeWaves> : pa_tree_kernel<KVT, D, NQ, 1>), grid,
-                     dim3(64 * kTreeWaves), 0, st, a);
+  constexpr int MT = tree_wave_tiles(D, NQ);
+  const dim3 threads(64 * kTreeWaves);
+  if (tiles == 1)
+    hipLaunchKernelGGL((pa_tree_kernel<KVT, D, NQ, NP, kTreeWaves, 1>), grid, threads, 0, st, a);
+  else if (tiles == 4 * MT)
+    hipLaunchKernelGGL((pa_tree_kernel<KVT, D, NQ, NP, 1, MT>), grid, threads, 0, st, a);
+  else if constexpr (MT == 2)
+    hipLaunchKernelGGL((pa_tree_kernel<KVT, D, NQ, NP, 2, MT>), grid, threads, 0, st, a);
+  else
+    return hipErrorInvalidValue;
   return hipGetLastError();
 }
 
-template <int KVT, int NQ>
+template <int KVT, int NQ, int NP>
 hipError_t launch_tree_dim(const TreeArgs& a, int D, int tiles, dim3 grid, hipStream_t st) {
-  return D == 64    ? launch_tree_tiles<KVT, 64, NQ>(a, tiles, grid, st)
-         : D == 128 ? launch_tree_tiles<KVT, 128, NQ>(a, tiles, grid, st)
-                    : launch_tree_tiles<KVT, 256, NQ>(a, tiles, grid, st);
+  return D == 64    ? launch_tree_tiles<KVT, 64, NQ, NP>(a, tiles, grid, st)
+         : D == 128 ? launch_tree_tiles<KVT, 128, NQ, NP>(a, tiles, grid, st)
+                    : launch_tree_tiles<KVT, 256, NQ, NP>(a, tiles, grid, st);
 }
 
-// fp16 products: queries of 16 bits are one part, fp32 ones two.
+// Probabilities are two parts; for results in bf16 one of fp16: each is off by up to 2^-11, the
+// result's own rounding by 2^-8.
 template <int KVT>
 hipError_t launch_tree_parts(const TreeArgs& a, int D, int tiles, dim3 grid, hipStream_t st) {
-  return a.dtype == LLM_F32 ? launch_tree_dim<KVT, 2>(a, D, tiles, grid, st)
-                            : launch_tree_dim<KVT, 1>(a, D, tiles, grid, st);
+  return a.dtype == LLM_F32   ? launch_tree_dim<KVT, tree_parts(KVT, LLM_F32), 2>(a, D, tiles, grid, st)
+         : a.dtype == LLM_F16 ? launch_tree_dim<KVT, tree_parts(KVT, LLM_F16), 2>(a, D, tiles, grid, st)
+                              : launch_tree_dim<KVT, 1, KVT == LLM_BF16 ? 2 : 1>(a, D, tiles, grid, st);
 }
 
 }  // namespace

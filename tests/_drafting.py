@@ -130,7 +130,8 @@ def tree(q, cache, contexts, lens, mask, beams, sm_scale):
                 # A score is off by its queries' halves (2^-22 of each product) and an fp32 sum of D
                 # products (D / 2 roundings of 2^-24 on the way and back, taken as D), its exponent by the
                 # roundings of (s - m) in log2 units; e^x by two steps; a probability's halves by 2^-18
-                # (bf16, the coarser) at most, the sums over the keys by len roundings of 2^-24.
+                # (bf16, the coarser) at most, the sums over the keys by len roundings of 2^-24.  For
+                # results in bf16 over other pools a probability is one fp16: rounded by half a step, 2^-11.
                 mags = (k[see].abs() * x.abs()).sum(-1).max() * abs(sm_scale)
                 off = float(mags) * (2.0 ** -22 + (D + 4) * 2.0 ** -24) + \
                     4 * float(s.abs().max() + 1) * 2.0 ** -23 + 2.0 ** -22
@@ -138,7 +139,8 @@ def tree(q, cache, contexts, lens, mask, beams, sm_scale):
                 low = 2.0 ** -14 if cache.dtype == torch.float16 else 0.0
                 off += float((torch.where(k[see].abs() < low, k[see].abs(), 0.0) * x.abs()).sum(-1).max()
                              * abs(sm_scale))
-                share = 2 * off + 2.0 ** -18 + (int(see.sum()) + 16) * 2.0 ** -24
+                one = q.dtype == torch.bfloat16 and cache.dtype != torch.bfloat16
+                share = 2 * off + (2.0 ** -11 if one else 2.0 ** -18) + (int(see.sum()) + 16) * 2.0 ** -24
                 room_for[b, i, h] = share * (w[:, None] * v[see].abs()).sum(0) + 1e-30 + \
                     (w[:, None] * torch.where(v[see].abs() < low, v[see].abs(), 0.0)).sum(0)
     return out, room_for
