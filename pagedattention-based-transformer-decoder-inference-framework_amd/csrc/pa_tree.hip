@@ -8,42 +8,50 @@ namespace llm {
 namespace {
 
 constexpr int kMergeThreads = 256;
+constexpr int kWaveRows = 2048;
 
-// A row's parts, relative to the largest of their maxima.  A workgroup a row: D / 4 threads hold
-// its dims, the others the same of every (1024 / D)th part.
-template <int D>
+// A row's parts, relative to the largest of their maxima: `LANES` threads a row, D / 4 of which
+// hold its dims, the others the same of every (4 LANES / D)th part.  A wave a row where there are
+// rows enough to fill the card, else a workgroup a row.
+template <int D, int LANES>
 __global__ __launch_bounds__(kMergeThreads) void pa_tree_merge_kernel(TreeArgs a) {
-  constexpr int PER = D / 4, WAYS = kMergeThreads / PER;
-  __shared__ f32x4 s_x[WAYS][PER];
-  __shared__ float s_sum[WAYS];
-  const long long row = blockIdx.x;
+  constexpr int PER = D / 4, WAYS = LANES / PER, ROWS = kMergeThreads / LANES;
+  __shared__ f32x4 s_x[ROWS][WAYS][PER];
+  __shared__ float s_sum[ROWS][WAYS];
+  const int mine = threadIdx.x / LANES, d = threadIdx.x % PER, way = threadIdx.x % LANES / PER;
+  const long long row = (long long)blockIdx.x * ROWS + mine;
   const long long token = row / a.H;
   const int h = (int)(row - token * a.H), b = (int)(token / a.N), i = (int)(token - (long long)b * a.N);
-  const TreeRow tr = tree_row(a, b);
-  if (i >= tr.n) return;
-  const int parts = max((tr.L + tr.split_len - 1) / tr.split_len, 1);
-  const int d = threadIdx.x % PER, way = threadIdx.x / PER;
-  const float* ml = a.ml + (size_t)row * a.nsplit * 2;
-  const f32x4* acc = reinterpret_cast<const f32x4*>(a.acc + (size_t)row * a.nsplit * D) + d;
-  float M = kNegSentinel;
-  for (int s = lane_id(); s < parts; s += 64) M = fmaxf(M, ml[2 * s]);
-  M = wave_max(M);
+  bool live = row < (long long)a.B * a.N * a.H;
   float sum = 0.f;
   f32x4 x = {0.f, 0.f, 0.f, 0.f};
+  if (live) {
+    const TreeRow tr = tree_row(a, b);
+    live = i < tr.n;
+    const int parts = live ? max((tr.L + tr.split_len - 1) / tr.split_len, 1) : 0;
+    const float* ml = a.ml + (size_t)row * a.nsplit * 2;
+    const f32x4* acc = reinterpret_cast<const f32x4*>(a.acc + (size_t)row * a.nsplit * D) + d;
+    float M = kNegSentinel;
+    for (int s = lane_id(); s < parts; s += 64) M = fmaxf(M, ml[2 * s]);
+    M = wave_max(M);
 #pragma unroll 4
-  for (int s = way; s < parts; s += WAYS) {
-    const float weight = __builtin_amdgcn_exp2f(ml[2 * s] - M);
-    sum = fmaf(ml[2 * s + 1], weight, sum);
-    x += acc[(size_t)s * PER] * weight;
+    for (int s = way; s < parts; s += WAYS) {
+      const float weight = __builtin_amdgcn_exp2f(ml[2 * s] - M);
+      sum = fmaf(ml[2 * s + 1], weight, sum);
+      x += acc[(size_t)s * PER] * weight;
+    }
   }
-  s_x[way][d] = x;
-  if (d == 0) s_sum[way] = sum;
-  __syncthreads();
-  if (way > 0) return;
-  for (int v = 1; v < WAYS; ++v) {
-    x += s_x[v][d];
-    sum += s_sum[v];
+  if constexpr (WAYS > 1) {
+    s_x[mine][way][d] = x;
+    if (d == 0) s_sum[mine][way] = sum;
+    __syncthreads();
+    if (way > 0) return;
+    for (int v = 1; v < WAYS; ++v) {
+      x += s_x[mine][v][d];
+      sum += s_sum[mine][v];
+    }
   }
+  if (!live) return;
   x *= 1.f / (sum + 1e-6f);
   const size_t at = (size_t)token * a.out_stride + (size_t)h * D + 4 * d;
   if (a.dtype == LLM_F32) {
@@ -57,13 +65,29 @@ __global__ __launch_bounds__(kMergeThreads) void pa_tree_merge_kernel(TreeArgs a
   }
 }
 
+template <int D>
+hipError_t launch_merge(const TreeArgs& a, hipStream_t st) {
+  const long long rows = (long long)a.B * a.N * a.H;
+  if (rows >= kWaveRows)
+    hipLaunchKernelGGL((pa_tree_merge_kernel<D, 64>), dim3((unsigned)((rows + 3) / 4)), dim3(kMergeThreads), 0, st, a);
+  else
+    hipLaunchKernelGGL((pa_tree_merge_kernel<D, kMergeThreads>), dim3((unsigned)rows), dim3(kMergeThreads), 0, st, a);
+  return hipGetLastError();
+}
+
 struct TreePlan {
   int tiles;  // row tiles of a workgroup
   int row_groups, nsplit, split_keys;
 };
 
-// Splits: as many as bring the launch to about 1024 workgroups, none below 256 keys (the 4
-// waves' two blocks each).
+// Splits of equal length, as many as fill the card once: two workgroups a CU, one where heads of 256
+// leave registers for one (16 heads x 63 rows over 32768 e4m3 tokens, us: 256 workgroups 61, 512 54,
+// 1024 65; 8 x 16 heads of 256 over 4000 int8 tokens 256 31, 512 38).  A split has a fixed cost
+// of some 5 us and its parts' way through memory: none below 256 keys, 128 where a turn takes
+// four waves' tiles (4 x 80 rows over 1000 tokens 19, by 256 keys 23), and none of one tile's rows up
+// to 512 tokens (12 heads x 8 over 300 tokens 7.4, in two splits 9.6).  Where the rows alone fill
+// the card the parts are there against uneven rows: 2048 keys (64 x 16 heads over up to 8192 int8
+// tokens: whole rows 257 us, 4096 keys 245, 2048 233, 1024 240).
 TreePlan tree_plan(const pa_kv_view& kv, int dtype, int B, int N, int H, int T) {
   TreePlan p;
   const int rows = N * (H / kv.num_heads);
@@ -72,10 +96,13 @@ TreePlan tree_plan(const pa_kv_view& kv, int dtype, int B, int N, int H, int T) 
   const long long room = (long long)kv.max_tiles * kv.page_size;
   const long long keys = std::max(1LL, std::min((long long)T + N, room));
   const long long base = (long long)B * kv.num_heads * p.row_groups;
-  const long long want = std::max(1LL, 1024 / base);
-  long long per = (keys + want - 1) / want;
-  per = std::max(256LL, (per + kTreeStep - 1) / kTreeStep * kTreeStep);
-  p.split_keys = (int)std::min(per, (long long)1 << 30);
+  const long long fill = kv.head_dim == 256 ? 256 : 512;
+  const bool one = p.tiles == 1;
+  const long long least = base >= fill ? 2048 : one ? (keys <= 512 ? 512 : 256) : 128;
+  const long long want = base >= fill ? keys : fill / base;
+  long long per = std::max(least, (keys + want - 1) / want);
+  per = (per + kTreeStep - 1) / kTreeStep * kTreeStep;
+  p.split_keys = (int)std::min(per, 1LL << 30);
   p.nsplit = (int)std::min((keys + per - 1) / per, 1024LL);
   return p;
 }
@@ -176,14 +203,7 @@ extern "C" int pa_tree(const pa_kv_view* kv, const pa_kv_scales* scales, const v
                                             : launch_tree_e4m3(a, D, p.tiles, grid, st);
   LLM_HIP_RET(e);
   if (p.nsplit > 1) {
-    const dim3 rows((unsigned)((long long)B * N * H));
-    if (D == 64)
-      hipLaunchKernelGGL(pa_tree_merge_kernel<64>, rows, dim3(kMergeThreads), 0, st, a);
-    else if (D == 128)
-      hipLaunchKernelGGL(pa_tree_merge_kernel<128>, rows, dim3(kMergeThreads), 0, st, a);
-    else
-      hipLaunchKernelGGL(pa_tree_merge_kernel<256>, rows, dim3(kMergeThreads), 0, st, a);
-    LLM_HIP_RET(hipGetLastError());
+    LLM_HIP_RET(D == 64 ? launch_merge<64>(a, st) : D == 128 ? launch_merge<128>(a, st) : launch_merge<256>(a, st));
   }
   return LLM_OK;
 }

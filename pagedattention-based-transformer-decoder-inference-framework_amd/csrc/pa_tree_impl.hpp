@@ -15,8 +15,10 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 // Operands of 16 bits, as the products of one pool type take them.
 template <bool BF>
 struct Half {  // fp16
-  static constexpr float kP = 16384.f;    // probabilities enter times this
-  static constexpr float kGrow = 1.f;     // a maximum moves when it grew by more (log2 units)
+  // Probabilities enter times kP; a maximum moves when it grew by more than kGrow (log2 units), so
+  // that they stay below 2^15: what falls below fp16's normal numbers is 2^-25 of the largest.
+  static constexpr float kP = 2048.f;
+  static constexpr float kGrow = 4.f;
   static constexpr uint32_t kOne = 0x3c00u;
   static __device__ __forceinline__ f32x4 dot(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
@@ -150,15 +152,22 @@ __global__ __launch_bounds__(64 * kTreeWaves, D <= 128 ? 2 : 1) void pa_tree_ker
   const int32_t* pt = a.table + ((size_t)(has_beam ? beam : 0) * a.kv_heads + kvh) * a.max_tiles;
   const int blocks = (hi - lo + kTreeKeys - 1) / kTreeKeys;
 
-  // Lane i: the page of 16 keys (-1: none) and where in it they begin, of the 64 halves from block
-  // `from` on: this wave's own blocks, or, staged, all.
+  // Lane i: where 16 keys lie, of the 64 halves from block `from` on: this wave's own blocks, or,
+  // staged, all.
   constexpr int LOOKED = STAGED ? 32 / KW : 32;  // turns of a look-up
-  int pages, slots;
+  bool found;
+  uint64_t at_pool, at_scale;  // bytes into the pools, into the scales (of page 0 where there is none: masked)
   auto look_up = [&](int key) {
-    const int tile = key / a.page_size;
-    slots = key - tile * a.page_size;
+    const int tile = key / a.page_size, slot = key - tile * a.page_size;
     const int p = has_beam && key < hi ? pt[tile] : -1;
-    pages = p >= 0 && p < a.num_pages ? p : -1;
+    found = p >= 0 && p < a.num_pages;
+    const uint64_t page = found ? p : 0;
+    at_pool = page * a.page_stride + (uint32_t)slot * ROWB;
+    at_scale = (page * a.scale_stride + (uint32_t)slot) * 4;
+  };
+  auto lane64 = [](uint64_t x, int lane) {
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), lane) << 32 |
+           (uint32_t)__builtin_amdgcn_readlane((int)x, lane);
   };
   auto look_up_from = [&](int i) {
     look_up(STAGED ? lo + i * KW * kTreeKeys + 16 * lane
@@ -176,32 +185,26 @@ __global__ __launch_bounds__(64 * kTreeWaves, D <= 128 ? 2 : 1) void pa_tree_ker
     f32x4 ks[2], vs[2];
     uint32_t here;  // bit u: its u-th 16 keys have a page
   };
-  auto load_scales = [&](Block& x, int u, int page, int slot) {
-    if constexpr (QUANT) {
-      if (a.k_scale) {
-        const size_t s = (size_t)page * a.scale_stride + slot;
-        const float *ks = a.k_scale + s, *vs = a.v_scale + s;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          x.ks[u][r] = ks[4 * g + r];
-          x.vs[u][r] = vs[4 * g + r];
-        }
-      } else {
-        x.ks[u] = x.vs[u] = f32x4{1.f, 1.f, 1.f, 1.f};
-      }
-    }
-  };
   auto load = [&](Block& x, int i) {  // this wave's i-th block
-    x.here = 0;
+    x.here = (uint32_t)(__ballot(found) >> half_of(i, 0, 0)) & 3u;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const int found = __builtin_amdgcn_readlane(pages, half_of(i, 0, u));
-      x.here |= (found >= 0 ? 1u : 0u) << u;
-      const int page = max(found, 0);  // (what is read of page 0 instead is masked)
-      const int slot = __builtin_amdgcn_readlane(slots, half_of(i, 0, u));
-      load_scales(x, u, page, slot);
-      const size_t base = (size_t)page * a.page_stride + (size_t)slot * ROWB;
+      const uint64_t base = lane64(at_pool, half_of(i, 0, u));
       const uint8_t *kp = a.k_pool + base, *vp = a.v_pool + base;
+      if constexpr (QUANT) {
+        if (a.k_scale) {
+          const uint64_t at = lane64(at_scale, half_of(i, 0, u));
+          const float* ks = reinterpret_cast<const float*>(reinterpret_cast<const uint8_t*>(a.k_scale) + at);
+          const float* vs = reinterpret_cast<const float*>(reinterpret_cast<const uint8_t*>(a.v_scale) + at);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            x.ks[u][r] = ks[4 * g + r];
+            x.vs[u][r] = vs[4 * g + r];
+          }
+        } else {
+          x.ks[u] = x.vs[u] = f32x4{1.f, 1.f, 1.f, 1.f};
+        }
+      }
 #pragma unroll
       for (int l = 0; l < NKL; ++l)
         x.k[u][l] = *reinterpret_cast<const u32x4*>(kp + (uint32_t)(c * ROWB + 64 * l + 16 * g));
@@ -233,35 +236,29 @@ __global__ __launch_bounds__(64 * kTreeWaves, D <= 128 ? 2 : 1) void pa_tree_ker
            : CPR == 16 ? (key << 1 | key >> 3) & 15
                        : key & 15;
   };
-  auto stage = [&](int i) {
+  auto stage = [&](int i, int slot) {  // (slot: i % STAGES)
 #pragma unroll
     for (int j = 0; j < kStage / 1024 / kTreeWaves; ++j) {
       const int at = j * kTreeWaves + w;               // of the instructions
       const int block = at / (kBlock / 1024);
       const int row = at * (1024 / ROWB) % kTreeKeys;  // its first
-      const int half = half_of(i, block, row >> 4);
-      const int page = max(__builtin_amdgcn_readlane(pages, half), 0);
-      const int slot = __builtin_amdgcn_readlane(slots, half);
       const uint8_t* pool = at % (kBlock / 1024) < kBlock / 2048 ? a.k_pool : a.v_pool;
       const int key = (row & 15) + lane / CPR;
-      load_to_lds(pool + (size_t)page * a.page_stride + (size_t)slot * ROWB +
+      load_to_lds(pool + lane64(at_pool, half_of(i, block, row >> 4)) +
                       (uint32_t)(key * ROWB + 16 * (lane % CPR ^ exchange(key))),
-                  s_mem + i % STAGES * kStage + at * 1024);
+                  s_mem + slot * kStage + at * 1024);
     }
     if constexpr (QUANT) {  // this wave's block, lane l: of key l % 32
-      const int h0 = half_of(i, kw, 0), h1 = half_of(i, kw, 1);
-      const int p0 = __builtin_amdgcn_readlane(pages, h0), p1 = __builtin_amdgcn_readlane(pages, h1);
-      const int s0 = __builtin_amdgcn_readlane(slots, h0), s1 = __builtin_amdgcn_readlane(slots, h1);
-      const int u = lane >> 4 & 1;
+      const uint64_t s0 = lane64(at_scale, half_of(i, kw, 0)), s1 = lane64(at_scale, half_of(i, kw, 1));
       // (without scales anything, so that a stage has the same number of loads)
-      const float* src = reinterpret_cast<const float*>(a.k_pool);
+      const uint8_t* src = a.k_pool;
       if (a.k_scale)
-        src = (lane < 32 ? a.k_scale : a.v_scale) + (size_t)max(u ? p1 : p0, 0) * a.scale_stride + (u ? s1 : s0) + c;
-      load_to_lds_dword(src, s_mem + STAGES * kStage + i % STAGES * kScales + w * 256);
+        src = reinterpret_cast<const uint8_t*>(lane < 32 ? a.k_scale : a.v_scale) + (lane & 16 ? s1 : s0) + 4 * c;
+      load_to_lds_dword(src, s_mem + STAGES * kStage + slot * kScales + w * 256);
     }
   };
-  auto fetch = [&](Block& x, int i) {  // this wave's block of turn i
-    const uint8_t* k = s_mem + i % STAGES * kStage + kw * kBlock;
+  auto fetch = [&](Block& x, int slot) {  // this wave's block of the turn
+    const uint8_t* k = s_mem + slot * kStage + kw * kBlock;
     const uint8_t* v = k + kBlock / 2;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
@@ -290,7 +287,7 @@ __global__ __launch_bounds__(64 * kTreeWaves, D <= 128 ? 2 : 1) void pa_tree_ker
         }
       }
       if constexpr (QUANT) {
-        const float* s = reinterpret_cast<const float*>(s_mem + STAGES * kStage + i % STAGES * kScales + w * 256) +
+        const float* s = reinterpret_cast<const float*>(s_mem + STAGES * kStage + slot * kScales + w * 256) +
                          16 * u + 4 * g;
         const f32x4 one = {1.f, 1.f, 1.f, 1.f};
         x.ks[u] = a.k_scale ? *reinterpret_cast<const f32x4*>(s) : one;
@@ -303,6 +300,7 @@ __global__ __launch_bounds__(64 * kTreeWaves, D <= 128 ? 2 : 1) void pa_tree_ker
   u32x4 q[MT][NQ][NK];
   float qf[MT];  // what its scores are multiplied by, in log2 units: > 0, so that -infinity stays what it is
   int tok[MT];
+  auto queries = [&] {
 #pragma unroll
   for (int t = 0; t < MT; ++t) {
     const bool ok = c < rows_of(t);
@@ -357,11 +355,12 @@ __global__ __launch_bounds__(64 * kTreeWaves, D <= 128 ? 2 : 1) void pa_tree_ker
         for (int p = 0; p < NQ; ++p) q[t][p][kk][i] = part[p];
       }
   }
+  };
 
   f32x4 o[MT][ND];
   float m[MT], top[MT], l[MT];  // what p is relative to, the maximum (m <= top <= m + kGrow), the sum
   // of the values' scales: a power of two, at least the largest met; what a probability is multiplied by
-  float unit = 0x1p-100f, per_unit = QUANT ? 0x1p100f * Hf::kP : Hf::kP;
+  float unit = 0x1p-100f, per_unit = 0x1p100f * Hf::kP;
 #pragma unroll
   for (int t = 0; t < MT; ++t) {
     m[t] = top[t] = kNegSentinel;
@@ -426,6 +425,100 @@ __global__ __launch_bounds__(64 * kTreeWaves, D <= 128 ? 2 : 1) void pa_tree_ker
           unusable |= !all;
         }
     }
+    // Scores, in a block of code of its own with their maxima: all tiles' products side by side.
+    f32x4 s[MT][2];
+    {
+      u32x4 kf[2][NK];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int kk = 0; kk < NK; ++kk) {
+          if constexpr (QUANT) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const uint32_t y = x.k[u][kk / 2][2 * (kk & 1) + e] ^ (KVT == LLM_I8 ? 0x80808080u : 0u);
+              kf[u][kk][2 * e] = two_codes<KVT, false>(y);
+              kf[u][kk][2 * e + 1] = two_codes<KVT, true>(y);
+            }
+          } else {
+            kf[u][kk] = x.k[u][kk];
+          }
+        }
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) s[t][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int p = 0; p < NQ; ++p)
+#pragma unroll
+        for (int kk = 0; kk < NK; ++kk)
+#pragma unroll
+          for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) s[t][u] = Hf::dot(kf[u][kk], q[t][p][kk], s[t][u]);
+    }
+    if constexpr (QUANT) {
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) s[t][u] *= x.ks[u];
+    }
+    uint32_t seen[MT];
+    if (special) {
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        seen[t] = present & visible(tok[t], key0);
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (!(seen[t] >> (16 * u + 4 * g + r) & 1u)) s[t][u][r] = -INFINITY;
+      }
+    }
+    bool grown = false;
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+      float most = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) most = fmaxf(most, s[t][u][r]);
+      top[t] = fmaxf(top[t], rows_max(most) * qf[t]);
+      grown |= top[t] > m[t] + Hf::kGrow;
+    }
+    if constexpr (QUANT) {
+      float most = 0.f;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) most = fmaxf(most, fabsf(x.vs[u][r]));
+      grown |= most > unit;
+    }
+    if (__any(grown)) {  // few blocks: sums move to the new maxima, and to the new unit of scales
+      float down = 1.f;
+      if constexpr (QUANT) {
+        float most = 0.f;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (fabsf(x.vs[u][r]) < INFINITY) most = fmaxf(most, fabsf(x.vs[u][r]));
+        int e = 0;
+        (void)frexpf(rows_max(most), &e);
+        const float next = fmaxf(unit, ldexpf(1.f, min(e, 126)));
+        down = unit / next;
+        per_unit = Hf::kP / next;
+        unit = next;
+      }
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        const float corr = __builtin_amdgcn_exp2f(m[t] - top[t]);
+        l[t] *= corr;
+#pragma unroll
+        for (int dd = 0; dd < ND; ++dd) o[t][dd] *= corr * down;
+        m[t] = top[t];
+      }
+    }
     // V^T: the 8 keys' dims exchanged to 8 keys of one dim
     u32x4 vf[ND];
 #pragma unroll
@@ -448,91 +541,27 @@ __global__ __launch_bounds__(64 * kTreeWaves, D <= 128 ? 2 : 1) void pa_tree_ker
             vf[2 * e + 1][2 * u + hf] = __builtin_amdgcn_perm(v1, v0, 0x07060302u);
           }
         }
-    u32x4 kf[2][NK];
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int kk = 0; kk < NK; ++kk) {
-        if constexpr (QUANT) {
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const uint32_t y = x.k[u][kk / 2][2 * (kk & 1) + e] ^ (KVT == LLM_I8 ? 0x80808080u : 0u);
-            kf[u][kk][2 * e] = two_codes<KVT, false>(y);
-            kf[u][kk][2 * e + 1] = two_codes<KVT, true>(y);
-          }
-        } else {
-          kf[u][kk] = x.k[u][kk];
-        }
-      }
+    f32x4 vs[MT][2];  // what probabilities are multiplied by
     if constexpr (QUANT) {
-      float most = 0.f;
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < 2; ++u) {
+        x.vs[u] *= per_unit;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) most = fmaxf(most, fabsf(x.vs[u][r]));
-      if (__any(most > unit)) {
-        most = 0.f;
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (fabsf(x.vs[u][r]) < INFINITY) most = fmaxf(most, fabsf(x.vs[u][r]));
-        int e = 0;
-        (void)frexpf(fmaxf(rows_max(most), unit * 0.75f), &e);
-        const float next = ldexpf(1.f, min(e, 126)), down = unit / next;
-        per_unit = Hf::kP / next;
+        for (int t = 0; t < MT; ++t) vs[t][u] = x.vs[u];
+      }
+      if (special) {  // (the scale of what is not seen may be NaN)
 #pragma unroll
         for (int t = 0; t < MT; ++t)
 #pragma unroll
-          for (int dd = 0; dd < ND; ++dd) o[t][dd] *= down;
-        unit = next;
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (!(seen[t] >> (16 * u + 4 * g + r) & 1u)) vs[t][u][r] = 0.f;
       }
-      x.vs[0] *= per_unit;
-      x.vs[1] *= per_unit;
     }
+    u32x4 ph[MT][NP];
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
-      if (t > 0 && rows_of(t) <= 0) break;
-      f32x4 s[2], vs[2];
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int p = 0; p < NQ; ++p)
-#pragma unroll
-          for (int kk = 0; kk < NK; ++kk) s[u] = Hf::dot(kf[u][kk], q[t][p][kk], s[u]);
-        if constexpr (QUANT) {
-          s[u] *= x.ks[u];
-          vs[u] = x.vs[u];
-        }
-      }
-      if (special) {
-        const uint32_t seen = present & visible(tok[t], key0);
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const bool see = seen >> (16 * u + 4 * g + r) & 1u;
-            if (!see) s[u][r] = -INFINITY;
-            if constexpr (QUANT)  // (the scale of what is not seen may be NaN)
-              if (!see) vs[u][r] = 0.f;
-          }
-      }
-      float most = -INFINITY;
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) most = fmaxf(most, s[u][r]);
-      most = rows_max(most) * qf[t];
-      top[t] = fmaxf(top[t], most);
-      if (__any(most > m[t] + Hf::kGrow)) {
-        const float corr = __builtin_amdgcn_exp2f(m[t] - top[t]);
-        l[t] *= corr;
-#pragma unroll
-        for (int dd = 0; dd < ND; ++dd) o[t][dd] *= corr;
-        m[t] = top[t];
-      }
-      u32x4 ph[NP];
+    for (int t = 0; t < MT; ++t)
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -541,20 +570,25 @@ __global__ __launch_bounds__(64 * kTreeWaves, D <= 128 ? 2 : 1) void pa_tree_ker
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const int r = 2 * hf + e;
-            p[e] = __builtin_amdgcn_exp2f(fmaf(s[u][r], qf[t], -m[t]));
+            p[e] = __builtin_amdgcn_exp2f(fmaf(s[t][u][r], qf[t], -m[t]));
             l[t] += p[e];
-            p[e] *= QUANT ? vs[u][r] : per_unit;
+            if constexpr (QUANT) {
+              p[e] *= vs[t][u][r];
+            } else if constexpr (Hf::kP != 1.f) {
+              p[e] *= Hf::kP;
+            }
           }
           uint32_t part[NP];
           split_parts<Hf, NP>(p[0], p[1], part);
 #pragma unroll
-          for (int i = 0; i < NP; ++i) ph[i][2 * u + hf] = part[i];
+          for (int i = 0; i < NP; ++i) ph[t][i][2 * u + hf] = part[i];
         }
 #pragma unroll
-      for (int dd = 0; dd < ND; ++dd)
+    for (int dd = 0; dd < ND; ++dd)
 #pragma unroll
-        for (int i = 0; i < NP; ++i) o[t][dd] = Hf::dot(vf[dd], ph[i], o[t][dd]);
-    }
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int i = 0; i < NP; ++i) o[t][dd] = Hf::dot(vf[dd], ph[t][i], o[t][dd]);
   };
 
   // Turns; staged, waves without rows, or without a block in the last one, take their part in the loads.
@@ -566,16 +600,18 @@ __global__ __launch_bounds__(64 * kTreeWaves, D <= 128 ? 2 : 1) void pa_tree_ker
     if constexpr (STAGED) {
       constexpr int LOADS = kStage / 1024 / kTreeWaves + (QUANT ? 1 : 0);  // of a wave and stage
       uint64_t there = 0, before = 0;  // the halves looked up last, and those before, that have a page
-      auto start = [&](int i) {
+      auto start = [&](int i, int slot) {
         if (i % LOOKED == 0) {
           if (i) look_up_from(i);
           before = there;
-          there = __ballot(pages >= 0);
+          there = __ballot(found);
         }
-        stage(i);
+        stage(i, slot);
       };
       const int ahead = min(STAGES - 1, mine);
-      for (int i = 0; i < ahead; ++i) start(i);
+      for (int i = 0; i < ahead; ++i) start(i, i);
+      queries();  // (while the first blocks come)
+      int slot = 0, next = STAGES - 1;
       for (int i = 0; i < mine; ++i) {
         if (i + STAGES - 1 <= mine)
           wait_lds_loads<LOADS*(STAGES - 2)>();
@@ -583,17 +619,20 @@ __global__ __launch_bounds__(64 * kTreeWaves, D <= 128 ? 2 : 1) void pa_tree_ker
           wait_lds_loads();
         barrier_only();  // block i has landed, block i - 1 is read out
         const int last = min(i + STAGES - 1, mine - 1);
-        if (i + STAGES - 1 < mine) start(last);
+        if (i + STAGES - 1 < mine) start(last, next);
         if (rows_of(0) > 0 && i * KW + kw < blocks) {
           x.here = (uint32_t)((last / LOOKED == i / LOOKED ? there : before) >> half_of(i, kw, 0)) & 3u;
-          fetch(x, i);
+          fetch(x, slot);
           attend(x, i);
         }
+        next = slot;
+        slot = slot + 1 == STAGES ? 0 : slot + 1;
       }
       __syncthreads();  // the sums take the blocks' place
     } else if constexpr (AHEAD) {
       Block y;
       load(x, 0);
+      queries();
       for (int i = 0; i < mine; i += 2) {
         if (i + 1 < mine) load(y, i + 1);
         attend(x, i);
@@ -605,6 +644,7 @@ __global__ __launch_bounds__(64 * kTreeWaves, D <= 128 ? 2 : 1) void pa_tree_ker
         attend(y, i + 1);
       }
     } else {
+      queries();
       for (int i = 0; i < mine; ++i) {
         if (i && (i & 31) == 0) look_up_from(i);
         load(x, i);
@@ -619,8 +659,7 @@ __global__ __launch_bounds__(64 * kTreeWaves, D <= 128 ? 2 : 1) void pa_tree_ker
         const int key0 = lo + (i * KW + kw) * kTreeKeys;
         if (key0 + kTreeKeys <= tr.C || key0 >= hi) continue;
         look_up(key0 + 16 * (lane & 1));
-        const int page[2] = {__builtin_amdgcn_readlane(pages, 0), __builtin_amdgcn_readlane(pages, 1)};
-        const uint32_t present = present_of((page[0] >= 0 ? 1u : 0u) | (page[1] >= 0 ? 2u : 0u), key0);
+        const uint32_t present = present_of((uint32_t)__ballot(found) & 3u, key0);
         u32x4 one[MT];
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
@@ -641,8 +680,7 @@ __global__ __launch_bounds__(64 * kTreeWaves, D <= 128 ? 2 : 1) void pa_tree_ker
             for (int s = 0; s < 2; ++s) {
               const int u = e / 2, key = 4 * g + 2 * (e % 2) + s;
               if (!(present >> (16 * u + key) & 1u)) continue;
-              const uint8_t* at = a.v_pool + (size_t)page[u] * a.page_stride +
-                                  (size_t)(__builtin_amdgcn_readlane(slots, u) + key) * ROWB + (c * ND + dd) * ES;
+              const uint8_t* at = a.v_pool + lane64(at_pool, u) + (uint32_t)(key * ROWB + (c * ND + dd) * ES);
               const uint32_t x = ES == 1 ? *at : *reinterpret_cast<const uint16_t*>(at);
               constexpr uint32_t kInf = Unusable<KVT>::kInf, kSign = ES == 1 ? 0x80u : 0x8000u;
               const bool bad = (x & kInf) == kInf, nan = ES == 1 ? bad : (x & (kSign - 1u)) > kInf;
