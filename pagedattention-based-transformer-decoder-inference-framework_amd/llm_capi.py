@@ -13,7 +13,6 @@ from __future__ import annotations
 
 import ctypes
 import os
-import struct
 from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
@@ -100,16 +99,18 @@ _SIGS = {
     "pa_decode_ex_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
     "pa_prefill": (c_int, [ctypes.POINTER(PaKvView), c_void_p, c_int, c_void_p, c_int, c_int,
                            c_int, c_int, c_float, c_void_p, c_size_t, c_void_p]),
-    # (the structures of these as byref() or as packed bytes)
-    "kv_quant_write": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_ll, c_void_p,
-                               c_void_p, c_void_p, c_int, c_int, c_void_p]),
-    "kv_quant_read": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_ll, c_void_p,
-                              c_void_p, c_void_p, c_int, c_int, c_void_p]),
-    "pa_tree_workspace_bytes": (c_size_t, [c_void_p, c_int, c_int, c_int, c_int]),
-    "pa_tree": (c_int, [c_void_p, c_void_p, c_void_p, c_ll, c_void_p, c_ll, c_int, c_void_p,
-                        c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float,
-                        c_void_p, c_size_t, c_void_p]),
-    "logits_adjust": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_ll, c_void_p, c_void_p]),
+    "kv_quant_write": (c_int, [ctypes.POINTER(PaKvView), ctypes.POINTER(PaKvScales), c_void_p,
+                               c_void_p, c_int, c_ll, c_void_p, c_void_p, c_void_p, c_int, c_int,
+                               c_void_p]),
+    "kv_quant_read": (c_int, [ctypes.POINTER(PaKvView), ctypes.POINTER(PaKvScales), c_void_p,
+                              c_void_p, c_int, c_ll, c_void_p, c_void_p, c_void_p, c_int, c_int,
+                              c_void_p]),
+    "pa_tree_workspace_bytes": (c_size_t, [ctypes.POINTER(PaKvView), c_int, c_int, c_int, c_int]),
+    "pa_tree": (c_int, [ctypes.POINTER(PaKvView), ctypes.POINTER(PaKvScales), c_void_p, c_ll,
+                        c_void_p, c_ll, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int,
+                        c_int, c_int, c_int, c_float, c_void_p, c_size_t, c_void_p]),
+    "logits_adjust": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_ll,
+                              ctypes.POINTER(LogitsRules), c_void_p]),
     "gemm_packed_bytes": (c_size_t, [c_int, c_int, c_int]),
     "gemm_pack_weights": (c_int, [c_int, c_void_p, c_void_p, c_int, c_int, c_void_p]),
     "i8_gemm": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
@@ -375,123 +376,30 @@ def pa_prefill(q, k_pool, v_pool, page_table, *, row, p0, sm_scale=1.0, out=None
     return out
 
 
-# PaKvView, PaKvScales and LogitsRules as bytes (a structure's constructor takes 1.4 us, its
-# packing 0.4: of a short step's 14 us a call on the host these and the checks took 9).
-_PACK_VIEW, _PACK_SCALES = struct.Struct("@PPP7iq").pack, struct.Struct("@PPq").pack
-_PACK_RULES = struct.Struct("@PqiPPPPPPPqiPiP").pack
-
-_value_dtypes = None
+_calls = None
 
 
-def _value_dtype(t, name):
-    global _value_dtypes
-    if _value_dtypes is None:
-        import torch
-        _value_dtypes = {torch.float32: LLM_F32, torch.float16: LLM_F16, torch.bfloat16: LLM_BF16}
-    dtype = _value_dtypes.get(t.dtype)
-    if dtype is None:
-        raise TypeError(f"{name} must be fp32, fp16 or bf16, not {t.dtype}")
-    return dtype
+def _torch_calls():
+    """The module llm_torch, whose calls check their tensors and reach the loaded library."""
+    global _calls
+    if _calls is None:
+        import torch  # noqa: F401  (what the module is linked against)
+        import llm_torch
+        lib = load()
+        llm_torch.bind(*(ctypes.cast(getattr(lib, name), c_void_p).value
+                         for name in ("kv_quant_write", "kv_quant_read", "pa_tree",
+                                      "pa_tree_workspace_bytes", "logits_adjust")))
+        _calls = llm_torch
+    return _calls
 
 
-def _array(t, dev, dtype, shape, name):
-    """Address of an array that a call reads: of `dtype` and `shape` (None: any), contiguous, on
-    device number dev.  None stays None."""
-    if t is None:
-        return None
-    if t.get_device() != dev:
-        raise ValueError(f"{name} is on {t.device}, not on the device of the call's other tensors")
-    if t.dtype is not dtype:
-        raise TypeError(f"{name} must be {dtype}, not {t.dtype}")
-    if shape is not None and t.shape != shape:
-        raise ValueError(f"{name} must have the shape {tuple(shape)}, not {tuple(t.shape)}")
-    if not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous")
-    return t.data_ptr()
-
-
-def _device(t):
-    """Number of a tensor's device, which has to be the current one."""
-    import torch
+def _raw_stream(t):
+    """The current stream of a tensor's device, which has to be the current one."""
+    from torch import _C
     dev = t.get_device()
-    if dev < 0 or dev != torch.cuda.current_device():
+    if dev < 0 or dev != _C._cuda_getDevice():
         raise ValueError(f"tensors on {t.device}: they have to be on the current device")
-    return dev
-
-
-def _token_rows(t, shape, name):
-    """Elements from token to token of [B][N][H][D] (a view of wider tokens, or contiguous)."""
-    B, N, H, D = shape
-    outer, step, head, one = t.stride()
-    if N == 1:
-        step = outer if B > 1 else H * D
-    if (one != 1 and D > 1) or (head != D and H > 1) or (B > 1 and N > 1 and outer != N * step) or step < H * D:
-        raise ValueError(f"{name} must be [B][N][H][D] with one step between tokens and whole heads in them")
-    return step
-
-
-def _paged(k_pool, v_pool, page_table, dev):
-    """The packed view of pools and table, and (beams, heads) of the table."""
-    import torch
-    shape, strides = k_pool.shape, k_pool.stride()
-    if v_pool.get_device() != dev or v_pool.shape != shape:
-        raise ValueError("k_pool and v_pool must be of one device and shape")
-    if page_table.dim() != 3:
-        raise ValueError("page_table must be [num_beams][num_heads][max_tiles]")
-    table = _array(page_table, dev, torch.int32, None, "page_table")
-    beams, heads, tiles = page_table.shape
-    if len(shape) != 3 or strides[1:] != (shape[2], 1) or v_pool.stride() != strides or \
-            v_pool.dtype is not k_pool.dtype:
-        kv_view(k_pool, v_pool, page_table)  # raises, or a dimension of 1 has a step of its own
-    pages, ts, D = shape
-    kind = kv_dtype_of(k_pool)
-    step = 0 if strides[0] == ts * D or pages == 1 else strides[0] * k_pool.element_size()
-    return _PACK_VIEW(k_pool.data_ptr(), v_pool.data_ptr(), table, pages, ts, D, beams, heads, tiles, kind,
-                      step), beams, heads
-
-
-def _scales(k_pool, k_scale, v_scale, dev):
-    import torch
-    shape, strides = k_scale.shape, k_scale.stride()
-    for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
-        if t.dtype is not torch.float32:
-            raise TypeError(f"{name} must be fp32, not {t.dtype}")
-        if t.get_device() != dev:
-            raise ValueError(f"{name} is on {t.device}, not on {k_pool.device}")
-    if shape != k_pool.shape[:2] or v_scale.shape != shape or (strides[1] != 1 and shape[1] > 1):
-        raise ValueError("scales must be [num_pages][page_size] with contiguous pages")
-    if v_scale.stride() != strides:
-        raise ValueError("k_scale and v_scale must share one page stride")
-    return _PACK_SCALES(k_scale.data_ptr(), v_scale.data_ptr(), strides[0] if shape[0] > 1 else 0)
-
-
-def kv_scales(k_pool, k_scale, v_scale) -> PaKvScales:
-    """Scales fp32 [num_pages][page_size] of quantised pools [num_pages][page_size][D]; pages
-    of scales may be strided (both the same)."""
-    return PaKvScales.from_buffer_copy(_scales(k_pool, k_scale, v_scale, k_pool.get_device()))
-
-
-def _quant_call(entry, k, v, k_pool, v_pool, page_table, k_scale, v_scale, starts, lens, beam_ids, stream):
-    import torch
-    dev = _device(k_pool)
-    view, beams, heads = _paged(k_pool, v_pool, page_table, dev)
-    shape = k.shape
-    B, N, H, D = shape
-    if v.shape != shape or v.dtype is not k.dtype or H != heads or D != k_pool.shape[2]:
-        raise ValueError("k and v must be [B][N][num_heads][head_dim] of one type, as the pages are")
-    step = _token_rows(k, shape, "k")
-    if v.stride() != k.stride() and _token_rows(v, shape, "v") != step:
-        raise ValueError("k and v must have one step between tokens")
-    if k.get_device() != dev or v.get_device() != dev:
-        raise ValueError(f"k and v have to be on {k_pool.device}, as the pages are")
-    if beam_ids is None and B > beams:
-        raise ValueError("more rows than page_table has beams")
-    i32 = torch.int32
-    rc = entry(view, _scales(k_pool, k_scale, v_scale, dev), k.data_ptr(), v.data_ptr(), _value_dtype(k, "k"),
-               step, _array(beam_ids, dev, i32, (B,), "beam_ids"), _array(starts, dev, i32, (B,), "starts"),
-               _array(lens, dev, i32, (B,), "lens"), B, N, _stream(stream))
-    if rc:
-        check(rc)
+    return _C._cuda_getCurrentRawStream(dev)
 
 
 def kv_quant_write(k, v, k_pool, v_pool, page_table, k_scale, v_scale, *, starts, lens=None,
@@ -500,25 +408,36 @@ def kv_quant_write(k, v, k_pool, v_pool, page_table, k_scale, v_scale, *, starts
     views of wider tokens, such as a fused projection's, are taken as they are), row b's token j
     at position starts[b] + j for j < lens[b].  Pools int8 or float8_e4m3fn [num_pages][ts][D],
     scales fp32 [num_pages][ts]; both are written in place."""
-    _quant_call(load().kv_quant_write, k, v, k_pool, v_pool, page_table, k_scale, v_scale, starts, lens,
-                beam_ids, stream)
+    if stream is not None:
+        import torch
+        with torch.cuda.stream(stream):
+            return kv_quant_write(k, v, k_pool, v_pool, page_table, k_scale, v_scale, starts=starts,
+                                  lens=lens, beam_ids=beam_ids)
+    rc = _torch_calls().quant(True, k, v, k_pool, v_pool, page_table, k_scale, v_scale, starts, lens,
+                              beam_ids, _raw_stream(k_pool))
+    if rc:
+        check(rc)
 
 
 def kv_quant_read(k_pool, v_pool, page_table, k_scale, v_scale, *, starts, N=None, lens=None,
                   beam_ids=None, dtype=None, out=None, stream=None):
     """Read N tokens a row back from starts[b] on: (k, v) [B][N][H][D] of dtype (default fp32).
     Tokens past lens[b] are left as they are in out = (k, v), 0 without it."""
-    import torch
     if stream is not None:  # (what is allocated here belongs to that stream)
+        import torch
         with torch.cuda.stream(stream):
             return kv_quant_read(k_pool, v_pool, page_table, k_scale, v_scale, starts=starts, N=N,
                                  lens=lens, beam_ids=beam_ids, dtype=dtype, out=out)
     if out is None:
+        import torch
         shape = (starts.shape[0], N, page_table.shape[1], k_pool.shape[2])
         make = torch.empty if lens is None else torch.zeros
         out = tuple(make(shape, dtype=dtype or torch.float32, device=k_pool.device) for _ in "kv")
-    _quant_call(load().kv_quant_read, *out, k_pool, v_pool, page_table, k_scale, v_scale, starts, lens,
-                beam_ids, None)
+    k, v = out
+    rc = _torch_calls().quant(False, k, v, k_pool, v_pool, page_table, k_scale, v_scale, starts, lens,
+                              beam_ids, _raw_stream(k_pool))
+    if rc:
+        check(rc)
     return out
 
 
@@ -553,39 +472,18 @@ def pa_tree(q, k_pool, v_pool, page_table, *, T, context_lens=None, tree_mask=No
     drafted tokens of each row.  scales = (k_scale, v_scale) of quantised pools.  T bounds the
     committed tokens.  Returns out [B][N][H][D] of q's type; rows past tree_lens[b] are
     left as they are in `out`, 0 without it."""
-    import torch
     if stream is not None:
+        import torch
         with torch.cuda.stream(stream):
             return pa_tree(q, k_pool, v_pool, page_table, T=T, context_lens=context_lens,
                            tree_mask=tree_mask, tree_lens=tree_lens, beam_ids=beam_ids, scales=scales,
                            sm_scale=sm_scale, out=out)
-    lib = load()
-    dev = _device(k_pool)
-    view, beams, _ = _paged(k_pool, v_pool, page_table, dev)
-    shape = q.shape
-    B, N, H, D = shape
-    dtype = _value_dtype(q, "q")
-    if q.get_device() != dev:
-        raise ValueError(f"q is on {q.device}, not on {k_pool.device}")
-    if out is None:
-        out = (torch.empty if tree_lens is None else torch.zeros)(shape, dtype=q.dtype, device=q.device)
-    elif out.shape != shape or out.dtype is not q.dtype or out.get_device() != dev:
-        raise ValueError("out must have q's shape, type and device")
-    if beam_ids is None and B > beams:
-        raise ValueError("more rows than page_table has beams")
-    i32 = torch.int32
-    need = lib.pa_tree_workspace_bytes(view, B, N, H, T)
-    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    rc = lib.pa_tree(view, None if scales is None else _scales(k_pool, *scales, dev), q.data_ptr(),
-                     _token_rows(q, shape, "q"), out.data_ptr(), _token_rows(out, shape, "out"), dtype,
-                     _array(beam_ids, dev, i32, (B,), "beam_ids"),
-                     _array(context_lens, dev, i32, (B,), "context_lens"),
-                     _array(tree_mask, dev, i32, (B, N, (N + 31) // 32), "tree_mask"),
-                     _array(tree_lens, dev, i32, (B,), "tree_lens"), B, N, H, D, T, sm_scale, _at(ws), need,
-                     _stream(None))
-    if rc:
-        check(rc)
-    return out
+    k_scale, v_scale = (None, None) if scales is None else scales
+    got = _torch_calls().tree(q, k_pool, v_pool, page_table, k_scale, v_scale, context_lens, tree_mask,
+                              tree_lens, beam_ids, T, sm_scale, out, _raw_stream(k_pool))
+    if got.__class__ is int:
+        check(got)
+    return got if out is None else out
 
 
 def pack_weights(W, dtype: int, stream=None):
@@ -685,62 +583,19 @@ def logits_adjust(logits, *, history=None, history_lens=None, prompt_lens=None, 
     tokens in the history; then - frequency * c - presence * (c > 0); fp32 [R] each.  bias_ids int32
     and bias fp32 [R][n] (or [n]).  allowed int32 words [M][ceil(V / 32)], bit v set: allowed, -inf
     else; allowed_rows int32 [R] the row's mask (-1: none; None: mask r)."""
-    import torch
     if stream is not None:
+        import torch
         with torch.cuda.stream(stream):
             return logits_adjust(logits, history=history, history_lens=history_lens,
                                  prompt_lens=prompt_lens, repetition=repetition, frequency=frequency,
                                  presence=presence, bias_ids=bias_ids, bias=bias, allowed=allowed,
                                  allowed_rows=allowed_rows, out=out)
-    dev = _device(logits)
-    R, V = shape = logits.shape
-    dtype = _value_dtype(logits, "logits")
-    step, one = logits.stride()
-    if R <= 1:
-        step = V
-    if (one != 1 and V > 1) or step < V:
-        raise ValueError("logits must be [R][V] with contiguous rows")
-    if out is None:
-        out = torch.empty_strided(shape, (step, 1), dtype=logits.dtype, device=logits.device)
-    elif out.shape != shape or out.dtype is not logits.dtype or out.get_device() != dev or \
-            (out.stride(1) != 1 and V > 1) or (R > 1 and out.stride(0) != step):
-        raise ValueError("out must have the logits' shape, type, strides and device")
-
-    def entries(t, name):  # of a row in [R][n] or [n], and from row to row
-        if t.dim() == 2 and t.shape[0] == R:
-            return t.shape[1], t.shape[1]
-        if t.dim() != 1:
-            raise ValueError(f"{name} must be [{R}][n] or [n]")
-        return t.shape[0], 0
-
-    f32, i32 = torch.float32, torch.int32
-    # (empty lists have no address)
-    L = history_step = n = bias_step = masks = 0
-    if history is not None:
-        L, history_step = entries(history, "history")
-    past = [_array(history, dev, i32, None, "history"), _array(history_lens, dev, i32, (R,), "history_lens"),
-            _array(prompt_lens, dev, i32, (R,), "prompt_lens"), _array(repetition, dev, f32, (R,), "repetition"),
-            _array(frequency, dev, f32, (R,), "frequency"), _array(presence, dev, f32, (R,), "presence")]
-    if history is not None and not L:
-        past = [None] * 6
-    if bias_ids is not None or bias is not None:
-        if bias_ids is None or bias is None or bias.shape != bias_ids.shape:
-            raise ValueError("bias_ids and bias go together, of one shape")
-        n, bias_step = entries(bias_ids, "bias_ids")
-    ids, values = _array(bias_ids, dev, i32, None, "bias_ids"), _array(bias, dev, f32, None, "bias")
-    if allowed is not None:
-        if allowed.dim() != 2 or allowed.shape[1] != (V + 31) // 32:
-            raise ValueError(f"allowed must be [masks][{(V + 31) // 32}]")
-        masks = allowed.shape[0]
-    given = [x or 0 for x in past + [ids if n else 0, values if n else 0,
-                                     _array(allowed, dev, i32, None, "allowed"),
-                                     _array(allowed_rows, dev, i32, (R,), "allowed_rows")]]
-    rc = load().logits_adjust(logits.data_ptr(), out.data_ptr(), dtype, R, V, step,
-                              _PACK_RULES(given[0], history_step, L, *given[1:8], bias_step, n, given[8], masks,
-                                          given[9]), _stream(None))
-    if rc:
-        check(rc)
-    return out
+    got = _torch_calls().adjust(logits, history, history_lens, prompt_lens, repetition, frequency,
+                                presence, bias_ids, bias, allowed, allowed_rows, out,
+                                _raw_stream(logits))
+    if got.__class__ is int:
+        check(got)
+    return got if out is None else out
 
 
 def quantize_rows(x, stream=None):

@@ -123,11 +123,21 @@ def test_tree_mask():
         llm_capi.tree_mask([-1, -2])
 
 
-def test_packed_structures():
-    """What the calls pack by hand has the structures' own layout."""
-    def same(kind, packed, values):
-        assert bytes(kind(*values)) == packed(*values) and ctypes.sizeof(kind) == len(packed(*values))
-
-    same(llm_capi.PaKvView, llm_capi._PACK_VIEW, (1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 1 << 40))
-    same(llm_capi.PaKvScales, llm_capi._PACK_SCALES, (1, 2, 1 << 40))
-    same(llm_capi.LogitsRules, llm_capi._PACK_RULES, (1, 1 << 40, 3, 4, 5, 6, 7, 8, 9, 10, 1 << 41, 12, 13, 14, 15))
+def test_torch_calls_refuse_before_any_launch():
+    """The tensors' own checks, on tensors of the CPU: no call gets as far as the library."""
+    calls = llm_capi._torch_calls()
+    pool, table = torch.zeros((4, 16, 64), dtype=torch.int8), torch.zeros((1, 2, 2), dtype=torch.int32)
+    scale, x = torch.zeros((4, 16)), torch.zeros((1, 1, 2, 64))
+    one = torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(ValueError, match="current device"):
+        llm_capi.kv_quant_write(x, x, pool, pool, table, scale, scale, starts=one)
+    with pytest.raises(ValueError, match="current device"):
+        llm_capi.pa_tree(x, pool, pool, table, T=1)
+    with pytest.raises(ValueError, match="current device"):
+        llm_capi.logits_adjust(scale)
+    with pytest.raises(ValueError):
+        calls.quant(True, x, x, pool, pool, table, scale, scale, one, None, None, 0)
+    with pytest.raises(ValueError):
+        calls.tree(x, pool, pool, table, None, None, None, None, None, None, 1, 1.0, None, 0)
+    with pytest.raises(ValueError):
+        calls.adjust(scale, *[None] * 11, 0)
