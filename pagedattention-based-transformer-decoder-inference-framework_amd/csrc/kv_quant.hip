@@ -9,10 +9,13 @@
 // are whole lines, and a single token's heads lie beside each other in k and v.
 //
 // Codes are those of exact arithmetic.  c x in fp32, c = fp32(largest / a), is off by two
-// roundings, 2^-23 of itself, which matters where it is that near the border between two
-// codes: the codes of c x (1 +- 2^-21) are then two, and which one is right is asked in
-// fp64, where largest |x| and border * a are exact (24 + 9 bits).  About one element in ten
-// thousand asks.
+// roundings, 2^-23 of itself, which matters where it is that near the border between two codes:
+// there the question is asked in fp64, where largest |x| and border * a are exact (24 + 9 bits).
+// About one element in ten thousand asks.
+//
+// Bound by the bytes where there are many rows (4 x 4096 tokens of 16 heads of 128 from fp16 to int8
+// and back: written 45 us, read 40; 171 MB each way at the rate of a copy are 35), by the chain
+// of lens, table and stores where there are few (64 single tokens: 3.4 and 3.2 us).
 #include "common.hpp"
 #include "paged_rows.hpp"
 
@@ -73,69 +76,98 @@ __device__ __forceinline__ void store8(void* base, long long at, const float (&x
   }
 }
 
-// The code of the nearest value, and the value a code stands for.
 template <int KVT>
-struct Code;
-template <>
-struct Code<LLM_I8> {
-  static constexpr float largest = 127.f;
-  static __device__ __forceinline__ int of(float y) { return (int)rintf(y); }
-  static __device__ __forceinline__ float value(int code) { return (float)code; }
-};
-template <>
-struct Code<LLM_E4M3> {
-  static constexpr float largest = 448.f;
-  static __device__ __forceinline__ int of(float y) {
-    return __builtin_amdgcn_cvt_pk_fp8_f32(y, y, 0, false) & 0xff;
-  }
-  static __device__ __forceinline__ float value(int code) {
-    return __builtin_amdgcn_cvt_f32_fp8(code, 0);
-  }
-};
+constexpr float largest_of() {
+  return KVT == LLM_I8 ? 127.f : 448.f;
+}
+__device__ __forceinline__ float e4m3_value(uint32_t code) { return __builtin_amdgcn_cvt_f32_fp8((int)code, 0); }
+
+// The code of |y| <= border or above, y = largest x / a in exact arithmetic: `low` and `low` + 1
+// are the codes of magnitudes around the border, halves go to the even one.
+__device__ __forceinline__ int exact_code(float x, float a, float largest, int low, double border) {
+  const double at = (double)largest * fabs((double)x), edge = border * (double)a;
+  return at > edge || (at == edge && (low & 1)) ? low + 1 : low;
+}
 
 // 8 codes of 8 elements (as 8 bytes) and the row's scale; every lane of the row calls it.
 template <int KVT>
-__device__ __forceinline__ u32x2 quantise(const float (&x)[kPer], int lpr, float& scale) {
-  using C = Code<KVT>;
+__device__ __forceinline__ u32x2 quantise(float (&x)[kPer], int lpr, float& scale) {
+  constexpr float largest = largest_of<KVT>();
   uint32_t top = 0;  // of the magnitudes' bits: an infinity is above every number, a NaN above it
 #pragma unroll
   for (int i = 0; i < kPer; ++i) top = max(top, __builtin_bit_cast(uint32_t, x[i]) & 0x7fffffffu);
-  for (int m = 1; m < lpr; m <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, m, 64));
-  const bool finite = top < 0x7f800000u;
-  const float a = __builtin_bit_cast(float, top);
-  scale = finite ? a / C::largest : __builtin_nanf("");
-  // (rows of less than 2^-60 are taken 2^80 times larger: largest / a stays a number)
-  const float up = a < 0x1p-60f ? 0x1p80f : 1.f;
-  const bool live = finite && a > 0.f;
-  const float c = live ? C::largest / (a * up) : 0.f;
-  int code[kPer];
-  bool near = false;
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const float y = live ? x[i] * up * c : 0.f;
-    code[i] = C::of(y * (1.f - 0x1p-21f));
-    near |= code[i] != C::of(y * (1.f + 0x1p-21f));
+  // (mirrors of 8 and 16 lanes: their halves hold the same by then)
+  if (lpr >= 2) top = max(top, (uint32_t)mov_lanes<0xB1>((int)top));
+  if (lpr >= 4) top = max(top, (uint32_t)mov_lanes<0x4E>((int)top));
+  if (lpr >= 8) top = max(top, (uint32_t)mov_lanes<0x141>((int)top));
+  if (lpr >= 16) top = max(top, (uint32_t)mov_lanes<0x140>((int)top));
+  if (lpr >= 32) {
+    const LanePair p = with_lane16(__builtin_bit_cast(float, top));
+    top = max(__builtin_bit_cast(uint32_t, p.a), __builtin_bit_cast(uint32_t, p.b));
   }
-  if (near) {
+  const bool finite = top < 0x7f800000u;
+  float a = __builtin_bit_cast(float, top);
+  scale = finite ? a / largest : __builtin_nanf("");
+  if (a < 0x1p-60f) {  // (largest / a stays a number; what it is times is exact)
+    a *= 0x1p80f;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) x[i] *= 0x1p80f;
+  }
+  if (!finite || a == 0.f) return u32x2{0u, 0u};
+  const float c = largest / a;
+  u32x2 w = {0u, 0u};
+  if constexpr (KVT == LLM_I8) {
+    float far = 0.f;
+    int code[kPer];
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const float y = x[i] * up * c;
-      const int other = C::of(y * (1.f + 0x1p-21f));
-      if (other == code[i]) continue;
-      // magnitudes: `code` is the smaller one's
-      const double border = 0.5 * ((double)fabsf(C::value(code[i])) + (double)fabsf(C::value(other)));
-      const double at = (double)C::largest * fabs((double)x[i]), edge = border * (double)a;
-      if (at > edge || (at == edge && (other & 1) == 0)) code[i] = other;
+      const float y = x[i] * c, q = rintf(y);
+      far = fmaxf(far, fabsf(y - q));
+      code[i] = (int)q;
+    }
+    if (far > 0.5f - 0x1p-14f) {  // (y is off by 127 * 2^-23 at most)
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const float y = fabsf(x[i] * c);
+        if (fabsf(y - rintf(y)) <= 0.5f - 0x1p-14f) continue;
+        const int low = (int)y, mag = exact_code(x[i], a, largest, low, low + 0.5);
+        code[i] = x[i] < 0.f ? -mag : mag;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) w[i / 4] |= (uint32_t)(code[i] & 0xff) << (8 * (i % 4));
+  } else {
+    u32x2 up;  // the codes of a little more: others where y is near a border
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float y[4], z[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float t = x[4 * i + e] * c;
+        y[e] = t * (1.f - 0x1p-21f);
+        z[e] = t * (1.f + 0x1p-21f);
+      }
+      w[i] = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false), true);
+      up[i] = __builtin_amdgcn_cvt_pk_fp8_f32(z[2], z[3], __builtin_amdgcn_cvt_pk_fp8_f32(z[0], z[1], 0, false), true);
+    }
+    if (w[0] != up[0] || w[1] != up[1]) {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const int sh = 8 * (i % 4);
+        const uint32_t low = w[i / 4] >> sh & 0x7fu, high = up[i / 4] >> sh & 0x7fu;
+        if (low == high) continue;
+        const double border = 0.5 * ((double)e4m3_value(low) + (double)e4m3_value(high));
+        const uint32_t code = exact_code(x[i], a, largest, (int)low, border);
+        w[i / 4] = (w[i / 4] & ~(0x7fu << sh)) | code << sh;
+      }
     }
   }
-  u32x2 w = {0u, 0u};
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) w[i / 4] |= (uint32_t)(code[i] & 0xff) << (8 * (i % 4));
   return w;
 }
 
 struct Place {
-  bool token;  // the row has this token
+  bool value_there;  // k and v have this element
+  bool token;  // ... and the row this token
   bool page;   // ... and it has a page
   size_t at;   // bytes into a pool
   size_t scale;
@@ -154,7 +186,8 @@ __device__ __forceinline__ Place place_of(const QuantArgs& a, int lpr_log, bool 
   const int beam = a.beam_ids ? a.beam_ids[b] : b;
   const int start = a.starts[b];
   Place p;
-  p.token = j < n && h < a.num_heads && lane * kPer < a.D;
+  p.value_there = j < a.N && h < a.num_heads && lane * kPer < a.D;
+  p.token = p.value_there && j < n;
   p.value = ((long long)b * a.N + j) * a.token_stride + (long long)h * a.D + lane * kPer;
   p.page = false;
   p.at = p.scale = 0;
@@ -185,7 +218,7 @@ template <typename T, int KVT>
 __global__ __launch_bounds__(kThreads) void kv_quant_write_kernel(QuantArgs a, int lpr_log) {
   const Place p = place_of(a, lpr_log, true);
   float k[kPer] = {}, v[kPer] = {};
-  if (p.token) {
+  if (p.value_there) {  // (they do not wait for lens)
     load8<T>(a.k, p.value, k);
     load8<T>(a.v, p.value, v);
   }
@@ -205,7 +238,7 @@ __device__ __forceinline__ void values(u32x2 w, float scale, float (&x)[kPer]) {
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const uint32_t byte = w[i / 4] >> (8 * (i % 4)) & 0xff;
-    x[i] = scale * (KVT == LLM_I8 ? (float)(int8_t)byte : Code<LLM_E4M3>::value((int)byte));
+    x[i] = scale * (KVT == LLM_I8 ? (float)(int8_t)byte : e4m3_value(byte));
   }
 }
 
