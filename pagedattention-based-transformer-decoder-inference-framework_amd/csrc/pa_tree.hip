@@ -77,7 +77,7 @@ hipError_t launch_merge(const TreeArgs& a, hipStream_t st) {
 
 struct TreePlan {
   int tiles;  // row tiles of a workgroup
-  int row_groups, nsplit, split_keys;
+  int row_groups, nsplit, split_keys, waves;
 };
 
 // Splits of equal length, as many as fill the card once: two workgroups a CU, one where heads of 256
@@ -88,6 +88,11 @@ struct TreePlan {
 // to 512 tokens (12 heads x 8 over 300 tokens 7.4, in two splits 9.6).  Where the rows alone fill
 // the card the parts are there against uneven rows: 2048 keys (64 x 16 heads over up to 8192 int8
 // tokens: whole rows 257 us, 4096 keys 245, 2048 233, 1024 240).
+//
+// One tile's rows of 64 to 511 pairs of long rows take workgroups of 8 waves, half as many splits
+// (4 x 16 heads over up to 8192 fp16 tokens 36.6 -> 32.7 us, 16 x 12 of 64 over 2048 int8, 8 tokens
+// each, 19.6 -> 16.4, no merge); others 4 (12 heads over 1200 int8 tokens 11.7, by 8 waves 12.2; 64 x
+// 16 heads over 500 20.2 and 26.2).
 TreePlan tree_plan(const pa_kv_view& kv, int dtype, int B, int N, int H, int T) {
   TreePlan p;
   const int rows = N * (H / kv.num_heads);
@@ -96,8 +101,9 @@ TreePlan tree_plan(const pa_kv_view& kv, int dtype, int B, int N, int H, int T) 
   const long long room = (long long)kv.max_tiles * kv.page_size;
   const long long keys = std::max(1LL, std::min((long long)T + N, room));
   const long long base = (long long)B * kv.num_heads * p.row_groups;
-  const long long fill = kv.head_dim == 256 ? 256 : 512;
   const bool one = p.tiles == 1;
+  p.waves = one && base >= 64 && base < 512 && keys > 512 ? tree_most_waves(kv.head_dim) : 4;
+  const long long fill = kv.head_dim == 256 || p.waves == 8 ? 256 : 512;
   const long long least = base >= fill ? 2048 : one ? (keys <= 512 ? 512 : 256) : 128;
   const long long want = base >= fill ? keys : fill / base;
   long long per = std::max(least, (keys + want - 1) / want);
@@ -193,6 +199,7 @@ extern "C" int pa_tree(const pa_kv_view* kv, const pa_kv_scales* scales, const v
   a.scale2 = sm_scale * kLog2e;
   a.nsplit = p.nsplit;
   a.split_keys = p.split_keys;
+  a.waves = p.waves;
   a.acc = static_cast<float*>(workspace);
   a.ml = a.acc + (size_t)B * N * H * p.nsplit * D;
   const hipStream_t st = as_stream(stream);

@@ -52,12 +52,12 @@ struct TreeArgs {
   int mask_words;
   int B, N, H, G, T;  // G = H / kv_heads
   float scale2;       // sm_scale log2(e)
-  int nsplit, split_keys;
+  int nsplit, split_keys, waves;
   float *acc, *ml;  // [row][split][D], [row][split][2], row = (b N + token) H + head
 };
 
-constexpr int kTreeWaves = 4, kTreeKeys = 32;
-constexpr int kTreeStep = kTreeWaves * kTreeKeys;
+constexpr int kTreeKeys = 32;
+constexpr int kTreeStep = 128;  // splits begin at multiples of it
 
 // Committed and all tokens of row b, its drafts, and the keys of one of its splits: nsplit of
 // them hold the row however long it is.
@@ -85,6 +85,9 @@ constexpr int tree_wave_tiles(int D, int parts) { return D * parts <= 128 ? 2 : 
 inline int tree_tiles(int D, int parts, int rows) {
   return rows <= 16 ? 1 : rows <= 64 ? 4 : 4 * tree_wave_tiles(D, parts);
 }
+
+// Most waves of a workgroup of one row tile (heads of 256 leave a SIMD registers for one).
+constexpr int tree_most_waves(int D) { return D == 256 ? 4 : 8; }
 
 // pa_tree_*.hip
 hipError_t launch_tree_f16(const TreeArgs& a, int D, int tiles, dim3 grid, hipStream_t st);

@@ -110,8 +110,8 @@ __device__ __forceinline__ uint32_t usable(uint32_t w) {
 
 // NQ, NP: parts of a query, of a probability; KW: waves that share the keys of the same rows, the others
 // have rows of their own; MT: row tiles of a wave.
-template <int KVT, int D, int NQ, int NP, int KW, int MT>
-__global__ __launch_bounds__(64 * kTreeWaves, D <= 128 ? 2 : 1) void pa_tree_kernel(TreeArgs a) {
+template <int KVT, int D, int NQ, int NP, int WAVES, int KW, int MT>
+__global__ __launch_bounds__(64 * WAVES, D <= 128 ? 8 / WAVES : 1) void pa_tree_kernel(TreeArgs a) {
   constexpr bool QUANT = Raw<KVT>::QUANT;
   constexpr int ES = Raw<KVT>::ES, ROWB = D * ES;
   using Hf = Half<KVT == LLM_BF16>;
@@ -119,18 +119,18 @@ __global__ __launch_bounds__(64 * kTreeWaves, D <= 128 ? 2 : 1) void pa_tree_ker
   constexpr int NKL = ROWB / 64;      // 16-byte loads of a key tile
   constexpr int ND = D / 16;          // tiles of the output, dims of a lane's keys
   constexpr int NV = ND * ES / 4;     // registers of them
-  constexpr int RW = kTreeWaves / KW; // waves with rows of their own
-  constexpr bool STAGED = KW < kTreeWaves;  // keys shared by waves come through LDS
+  constexpr int RW = WAVES / KW;      // waves with rows of their own
+  constexpr bool STAGED = KW < WAVES;  // keys shared by waves come through LDS
   constexpr bool AHEAD = ROWB < 512;  // a block ahead of the one in work fits the registers
   constexpr int CPR = ROWB / 16;      // 16-byte chunks of a key's row
   constexpr int kBlock = 2 * kTreeKeys * ROWB, kStage = KW * kBlock;  // bytes of a block's K and V, of KW blocks'
   static_assert(STAGED || MT == 1, "what is loaded ahead leaves no room for more tiles");
   // Loads into LDS reach its first 64 KiB: as many stages as fit there, with their scales behind them.
-  constexpr int kScales = QUANT ? kTreeWaves * 256 : 0;  // a wave's own 64: of K, of V
+  constexpr int kScales = QUANT ? WAVES * 256 : 0;  // a wave's own 64: of K, of V
   constexpr int STAGES = !STAGED ? 1 : 65536 / (kStage + kScales) < 8 ? 65536 / (kStage + kScales) : 8;
   static_assert(!STAGED || STAGES >= 2, "a stage ahead");
-  constexpr int kSums = kTreeWaves * 16 * (D + 4) * 4, kLoads = STAGED ? STAGES * (kStage + kScales) : 0;
-  __shared__ __align__(16) uint8_t s_mem[kLoads > kSums + 512 ? kLoads : kSums + 512];
+  constexpr int kSums = WAVES * 16 * (D + 4) * 4, kLoads = STAGED ? STAGES * (kStage + kScales) : 0;
+  __shared__ __align__(16) uint8_t s_mem[kLoads > kSums + WAVES * 128 ? kLoads : kSums + WAVES * 128];
   // behind the last block: the waves' sums
   float(*s_acc)[16][D + 4] = reinterpret_cast<float(*)[16][D + 4]>(s_mem);
   float(*s_ml)[16][2] = reinterpret_cast<float(*)[16][2]>(s_mem + kSums);
@@ -238,8 +238,8 @@ __global__ __launch_bounds__(64 * kTreeWaves, D <= 128 ? 2 : 1) void pa_tree_ker
   };
   auto stage = [&](int i, int slot) {  // (slot: i % STAGES)
 #pragma unroll
-    for (int j = 0; j < kStage / 1024 / kTreeWaves; ++j) {
-      const int at = j * kTreeWaves + w;               // of the instructions
+    for (int j = 0; j < kStage / 1024 / WAVES; ++j) {
+      const int at = j * WAVES + w;               // of the instructions
       const int block = at / (kBlock / 1024);
       const int row = at * (1024 / ROWB) % kTreeKeys;  // its first
       const uint8_t* pool = at % (kBlock / 1024) < kBlock / 2048 ? a.k_pool : a.v_pool;
@@ -598,7 +598,7 @@ __global__ __launch_bounds__(64 * kTreeWaves, D <= 128 ? 2 : 1) void pa_tree_ker
     look_up_from(0);
     Block x;
     if constexpr (STAGED) {
-      constexpr int LOADS = kStage / 1024 / kTreeWaves + (QUANT ? 1 : 0);  // of a wave and stage
+      constexpr int LOADS = kStage / 1024 / WAVES + (QUANT ? 1 : 0);  // of a wave and stage
       uint64_t there = 0, before = 0;  // the halves looked up last, and those before, that have a page
       auto start = [&](int i, int slot) {
         if (i % LOOKED == 0) {
@@ -701,7 +701,8 @@ __global__ __launch_bounds__(64 * kTreeWaves, D <= 128 ? 2 : 1) void pa_tree_ker
     }
 
   // The sums of a tile's waves, relative to the largest maximum of the row.
-  const int rr = threadIdx.x >> 4, part = threadIdx.x & 15;  // a row, ND of its dims
+  // a row, ND of its dims; the first 256 threads take a tile, the others the next
+  const int rr = threadIdx.x >> 4 & 15, part = threadIdx.x & 15, mine_of = threadIdx.x >> 8;
 #pragma unroll
   for (int t = 0; t < MT; ++t) {
   const float back = __builtin_amdgcn_exp2f(m[t] - top[t]);
@@ -720,9 +721,10 @@ __global__ __launch_bounds__(64 * kTreeWaves, D <= 128 ? 2 : 1) void pa_tree_ker
   }
   __syncthreads();
 #pragma unroll
-  for (int tile = 0; tile < RW; ++tile) {
+  for (int pair_of = 0; pair_of < RW; pair_of += WAVES / 4) {
+    const int tile = pair_of + mine_of;
     const int row = first + 16 * (tile + RW * t) + rr;
-    if (row >= all_rows) break;
+    if (tile >= RW || row >= all_rows) break;
     float M = kNegSentinel;
 #pragma unroll
     for (int v = tile * KW; v < tile * KW + KW; ++v) M = fmaxf(M, s_ml[v][rr][0]);
@@ -765,14 +767,15 @@ __global__ __launch_bounds__(64 * kTreeWaves, D <= 128 ? 2 : 1) void pa_tree_ker
 // tiles: row tiles of a workgroup (tree_tiles).
 template <int KVT, int D, int NQ, int NP>
 hipError_t launch_tree_tiles(const TreeArgs& a, int tiles, dim3 grid, hipStream_t st) {
-  constexpr int MT = tree_wave_tiles(D, NQ);
-  const dim3 threads(64 * kTreeWaves);
-  if (tiles == 1)
-    hipLaunchKernelGGL((pa_tree_kernel<KVT, D, NQ, NP, kTreeWaves, 1>), grid, threads, 0, st, a);
+  constexpr int MT = tree_wave_tiles(D, NQ), MOST = tree_most_waves(D);
+  if (tiles == 1 && a.waves == MOST)
+    hipLaunchKernelGGL((pa_tree_kernel<KVT, D, NQ, NP, MOST, MOST, 1>), grid, dim3(64 * MOST), 0, st, a);
+  else if (tiles == 1)
+    hipLaunchKernelGGL((pa_tree_kernel<KVT, D, NQ, NP, 4, 4, 1>), grid, dim3(256), 0, st, a);
   else if (tiles == 4 * MT)
-    hipLaunchKernelGGL((pa_tree_kernel<KVT, D, NQ, NP, 1, MT>), grid, threads, 0, st, a);
+    hipLaunchKernelGGL((pa_tree_kernel<KVT, D, NQ, NP, 4, 1, MT>), grid, dim3(256), 0, st, a);
   else if constexpr (MT == 2)
-    hipLaunchKernelGGL((pa_tree_kernel<KVT, D, NQ, NP, 2, MT>), grid, threads, 0, st, a);
+    hipLaunchKernelGGL((pa_tree_kernel<KVT, D, NQ, NP, 4, 2, MT>), grid, dim3(256), 0, st, a);
   else
     return hipErrorInvalidValue;
   return hipGetLastError();
