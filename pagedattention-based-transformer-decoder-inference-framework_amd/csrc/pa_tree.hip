@@ -3,6 +3,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <cmath>
 
 namespace llm {
 namespace {
@@ -144,7 +145,7 @@ extern "C" int pa_tree(const pa_kv_view* kv, const pa_kv_scales* scales, const v
   LLM_REQUIRE(kv->head_dim == D, "pa_tree: D != kv->head_dim");
   LLM_REQUIRE(H % kv->num_heads == 0, "pa_tree: H must be a multiple of kv->num_heads");
   LLM_REQUIRE(value_size(dtype) > 0, "pa_tree: dtype must be LLM_F32, LLM_F16 or LLM_BF16");
-  LLM_REQUIRE(sm_scale == sm_scale && sm_scale - sm_scale == 0.f, "pa_tree: sm_scale must be finite");
+  LLM_REQUIRE(std::isfinite(sm_scale * kLog2e), "pa_tree: sm_scale must be finite");
   LLM_REQUIRE(kv->kv_dtype == LLM_I8 || (kv->kv_dtype == LLM_E4M3) == (scales != nullptr),
               "pa_tree: LLM_E4M3 pools need scales, 16-bit ones have none");
   if (D != 64 && D != 128 && D != 256)

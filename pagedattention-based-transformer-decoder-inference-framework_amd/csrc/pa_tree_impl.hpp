@@ -302,59 +302,59 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 8 / WAVES : 1) void pa_tree_
   int tok[MT];
   auto queries = [&] {
 #pragma unroll
-  for (int t = 0; t < MT; ++t) {
-    const bool ok = c < rows_of(t);
-    const int row = ok ? row_of(t) + c : 0;  // (no row: the first one's place, as zeros)
-    tok[t] = row / a.G;
-    const int h = kvh * a.G + row - tok[t] * a.G;
-    const size_t at = ((size_t)b * a.N + tok[t]) * a.q_stride + (size_t)h * D;
-    qf[t] = fmaxf(fabsf(a.scale2), 1e-37f);
-    float x[NK][8];
-    float most = 0.f;
+    for (int t = 0; t < MT; ++t) {
+      const bool ok = c < rows_of(t);
+      const int row = ok ? row_of(t) + c : 0;  // (no row: the first one's place, as zeros)
+      tok[t] = row / a.G;
+      const int h = kvh * a.G + row - tok[t] * a.G;
+      const size_t at = ((size_t)b * a.N + tok[t]) * a.q_stride + (size_t)h * D;
+      qf[t] = fmaxf(fabsf(a.scale2), 1e-37f);
+      float x[NK][8];
+      float most = 0.f;
 #pragma unroll
-    for (int kk = 0; kk < NK; ++kk) {
-      const int d = ES == 1 ? 64 * (kk / 2) + 16 * g + 8 * (kk & 1) : 32 * kk + 8 * g;
-      if (a.dtype == LLM_F32) {
-        const float* p = static_cast<const float*>(a.q) + at + d;
-        const f32x4 y = *reinterpret_cast<const f32x4*>(p), z = *reinterpret_cast<const f32x4*>(p + 4);
+      for (int kk = 0; kk < NK; ++kk) {
+        const int d = ES == 1 ? 64 * (kk / 2) + 16 * g + 8 * (kk & 1) : 32 * kk + 8 * g;
+        if (a.dtype == LLM_F32) {
+          const float* p = static_cast<const float*>(a.q) + at + d;
+          const f32x4 y = *reinterpret_cast<const f32x4*>(p), z = *reinterpret_cast<const f32x4*>(p + 4);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[kk][e] = y[e], x[kk][4 + e] = z[e];
-      } else {
-        const u32x4 y = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q) + at + d);
+          for (int e = 0; e < 4; ++e) x[kk][e] = y[e], x[kk][4 + e] = z[e];
+        } else {
+          const u32x4 y = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q) + at + d);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const f32x2 z = a.dtype == LLM_F16 ? Half<false>::values(y[e]) : Half<true>::values(y[e]);
-          x[kk][2 * e] = z[0], x[kk][2 * e + 1] = z[1];
+          for (int e = 0; e < 4; ++e) {
+            const f32x2 z = a.dtype == LLM_F16 ? Half<false>::values(y[e]) : Half<true>::values(y[e]);
+            x[kk][2 * e] = z[0], x[kk][2 * e + 1] = z[1];
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if (!ok) x[kk][e] = 0.f;
+          if (a.scale2 < 0.f) x[kk][e] = -x[kk][e];
+          most = fmaxf(most, fabsf(x[kk][e]));
         }
       }
+      if constexpr (KVT != LLM_BF16) {
+        int e = 0;
+        (void)frexpf(rows_max(most), &e);  // most < 2^e
+        e = clamp_int(e, -100, 128);
+        const float up = ldexpf(1.f, 14 - e);
+        qf[t] = fmaxf(qf[t] * ldexpf(1.f, e - 14), 1e-37f);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        if (!ok) x[kk][e] = 0.f;
-        if (a.scale2 < 0.f) x[kk][e] = -x[kk][e];
-        most = fmaxf(most, fabsf(x[kk][e]));
+        for (int kk = 0; kk < NK; ++kk)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[kk][i] *= up;
       }
-    }
-    if constexpr (KVT != LLM_BF16) {
-      int e = 0;
-      (void)frexpf(rows_max(most), &e);  // most < 2^e
-      e = clamp_int(e, -100, 100);
-      const float up = ldexpf(1.f, 14 - e);
-      qf[t] = fmaxf(qf[t] * ldexpf(1.f, e - 14), 1e-37f);
 #pragma unroll
       for (int kk = 0; kk < NK; ++kk)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[kk][i] *= up;
+        for (int i = 0; i < 4; ++i) {
+          uint32_t part[NQ];
+          split_parts<Hf, NQ>(x[kk][2 * i], x[kk][2 * i + 1], part);
+#pragma unroll
+          for (int p = 0; p < NQ; ++p) q[t][p][kk][i] = part[p];
+        }
     }
-#pragma unroll
-    for (int kk = 0; kk < NK; ++kk)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t part[NQ];
-        split_parts<Hf, NQ>(x[kk][2 * i], x[kk][2 * i + 1], part);
-#pragma unroll
-        for (int p = 0; p < NQ; ++p) q[t][p][kk][i] = part[p];
-      }
-  }
   };
 
   f32x4 o[MT][ND];
@@ -503,9 +503,10 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 8 / WAVES : 1) void pa_tree_
 #pragma unroll
           for (int r = 0; r < 4; ++r)
             if (fabsf(x.vs[u][r]) < INFINITY) most = fmaxf(most, fabsf(x.vs[u][r]));
+        most = rows_max(most);
         int e = 0;
-        (void)frexpf(rows_max(most), &e);
-        const float next = fmaxf(unit, ldexpf(1.f, min(e, 126)));
+        (void)frexpf(most, &e);  // most < 2^e
+        const float next = most > unit ? ldexpf(1.f, min(e, 126)) : unit;
         down = unit / next;
         per_unit = Hf::kP / next;
         unit = next;
@@ -705,62 +706,62 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 8 / WAVES : 1) void pa_tree_
   const int rr = threadIdx.x >> 4 & 15, part = threadIdx.x & 15, mine_of = threadIdx.x >> 8;
 #pragma unroll
   for (int t = 0; t < MT; ++t) {
-  const float back = __builtin_amdgcn_exp2f(m[t] - top[t]);
-  const float sum = add(with_lane32(add(with_lane16(l[t] * back))));
-  const float f = back * (QUANT ? unit / Hf::kP : 1.f / Hf::kP);
-  if (t) __syncthreads();  // the tiles before are read
+    const float back = __builtin_amdgcn_exp2f(m[t] - top[t]);
+    const float sum = add(with_lane32(add(with_lane16(l[t] * back))));
+    const float f = back * (QUANT ? unit / Hf::kP : 1.f / Hf::kP);
+    if (t) __syncthreads();  // the tiles before are read
 #pragma unroll
-  for (int r = 0; r < 4; ++r)
+    for (int r = 0; r < 4; ++r)
 #pragma unroll
-    for (int dd = 0; dd < ND; dd += 4)
-      *reinterpret_cast<f32x4*>(&s_acc[w][c][(4 * g + r) * ND + dd]) =
-          f32x4{o[t][dd][r] * f, o[t][dd + 1][r] * f, o[t][dd + 2][r] * f, o[t][dd + 3][r] * f};
-  if (g == 0) {
-    s_ml[w][c][0] = top[t];
-    s_ml[w][c][1] = sum;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int pair_of = 0; pair_of < RW; pair_of += WAVES / 4) {
-    const int tile = pair_of + mine_of;
-    const int row = first + 16 * (tile + RW * t) + rr;
-    if (tile >= RW || row >= all_rows) break;
-    float M = kNegSentinel;
-#pragma unroll
-    for (int v = tile * KW; v < tile * KW + KW; ++v) M = fmaxf(M, s_ml[v][rr][0]);
-    float all = 0.f, r[ND] = {};
-#pragma unroll
-    for (int v = tile * KW; v < tile * KW + KW; ++v) {
-      const float weight = __builtin_amdgcn_exp2f(s_ml[v][rr][0] - M);
-      all = fmaf(s_ml[v][rr][1], weight, all);
-#pragma unroll
-      for (int e = 0; e < ND; ++e) r[e] = fmaf(s_acc[v][rr][part * ND + e], weight, r[e]);
+      for (int dd = 0; dd < ND; dd += 4)
+        *reinterpret_cast<f32x4*>(&s_acc[w][c][(4 * g + r) * ND + dd]) =
+            f32x4{o[t][dd][r] * f, o[t][dd + 1][r] * f, o[t][dd + 2][r] * f, o[t][dd + 3][r] * f};
+    if (g == 0) {
+      s_ml[w][c][0] = top[t];
+      s_ml[w][c][1] = sum;
     }
-    const int token = row / a.G, h = kvh * a.G + row - token * a.G;
-    if (a.nsplit > 1) {
-      const size_t at = (((size_t)b * a.N + token) * a.H + h) * a.nsplit + split;
+    __syncthreads();
+#pragma unroll 1  // (a launch finds its code in no cache)
+    for (int pair_of = 0; pair_of < RW; pair_of += WAVES / 4) {
+      const int tile = pair_of + mine_of;
+      const int row = first + 16 * (tile + RW * t) + rr;
+      if (tile >= RW || row >= all_rows) break;
+      float M = kNegSentinel;
 #pragma unroll
-      for (int e = 0; e < ND; e += 4)
-        *reinterpret_cast<f32x4*>(a.acc + at * D + part * ND + e) = f32x4{r[e], r[e + 1], r[e + 2], r[e + 3]};
-      if (part == 0) {
-        a.ml[2 * at] = M;
-        a.ml[2 * at + 1] = all;
+      for (int v = tile * KW; v < tile * KW + KW; ++v) M = fmaxf(M, s_ml[v][rr][0]);
+      float all = 0.f, r[ND] = {};
+#pragma unroll
+      for (int v = tile * KW; v < tile * KW + KW; ++v) {
+        const float weight = __builtin_amdgcn_exp2f(s_ml[v][rr][0] - M);
+        all = fmaf(s_ml[v][rr][1], weight, all);
+#pragma unroll
+        for (int e = 0; e < ND; ++e) r[e] = fmaf(s_acc[v][rr][part * ND + e], weight, r[e]);
       }
-    } else {
-      const float inv = 1.f / (all + 1e-6f);
-      const size_t at = ((size_t)b * a.N + token) * a.out_stride + (size_t)h * D + part * ND;
+      const int token = row / a.G, h = kvh * a.G + row - token * a.G;
+      if (a.nsplit > 1) {
+        const size_t at = (((size_t)b * a.N + token) * a.H + h) * a.nsplit + split;
 #pragma unroll
-      for (int e = 0; e < ND; e += 4) {
-        const f32x4 y = f32x4{r[e], r[e + 1], r[e + 2], r[e + 3]} * inv;
-        if (a.dtype == LLM_F32)
-          *reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + at + e) = y;
-        else
-          *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(a.out) + at + e) =
-              a.dtype == LLM_F16 ? u32x2{Half<false>::pair(y[0], y[1]), Half<false>::pair(y[2], y[3])}
-                                 : u32x2{Half<true>::pair(y[0], y[1]), Half<true>::pair(y[2], y[3])};
+        for (int e = 0; e < ND; e += 4)
+          *reinterpret_cast<f32x4*>(a.acc + at * D + part * ND + e) = f32x4{r[e], r[e + 1], r[e + 2], r[e + 3]};
+        if (part == 0) {
+          a.ml[2 * at] = M;
+          a.ml[2 * at + 1] = all;
+        }
+      } else {
+        const float inv = 1.f / (all + 1e-6f);
+        const size_t at = ((size_t)b * a.N + token) * a.out_stride + (size_t)h * D + part * ND;
+#pragma unroll
+        for (int e = 0; e < ND; e += 4) {
+          const f32x4 y = f32x4{r[e], r[e + 1], r[e + 2], r[e + 3]} * inv;
+          if (a.dtype == LLM_F32)
+            *reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + at + e) = y;
+          else
+            *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(a.out) + at + e) =
+                a.dtype == LLM_F16 ? u32x2{Half<false>::pair(y[0], y[1]), Half<false>::pair(y[2], y[3])}
+                                   : u32x2{Half<true>::pair(y[0], y[1]), Half<true>::pair(y[2], y[3])};
+        }
       }
     }
-  }
   }
 }
 

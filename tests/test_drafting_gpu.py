@@ -342,6 +342,17 @@ def test_scores_and_scales_at_their_ends(gpu):
     check_tree(c, q, [290], None, None, None)
     c.scales[1].zero_()
     check_tree(c, q, [290], None, None, None)
+    # small value scales behind blocks that hold none, a first page that is missing, queries of any size
+    for cache in (I8, E4M3):
+        c = Cache(cache, 1, 1, 64, 16, 300, seed=33)
+        c.scales[1] *= 1e-6
+        c.table[0, 0, :4] = -1
+        check_tree(c, q, [290], None, None, None)
+        c.scales[1][c.table[0, 0, 4:9].long()] = 0.0
+        check_tree(c, q, [290], None, None, None)
+        check_tree(c, q.repeat(1, 1, 20, 1), [290], None, None, None)
+    c = Cache(F16, 1, 1, 64, 16, 300, seed=34)
+    check_tree(c, q * 1e32, [290], None, None, None, scale=1e-33)
     raw = Cache(I8, 1, 1, 64, 16, 300, seed=32)  # without scales: the codes themselves
     raw.scales = None
     check_tree(raw, q * 0.01, [290], None, None, None)
