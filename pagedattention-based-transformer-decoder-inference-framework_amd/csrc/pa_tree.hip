@@ -83,7 +83,8 @@ struct TreePlan {
 
 // Splits of equal length, as many as fill the card once: two workgroups a CU, one where heads of 256
 // leave registers for one (16 heads x 63 rows over 32768 e4m3 tokens, us: 256 workgroups 61, 512 54,
-// 1024 65; 8 x 16 heads of 256 over 4000 int8 tokens 256 31, 512 38).  A split has a fixed cost
+// 1024 65; 8 x 16 heads of 256 over 4000 int8 tokens 256 31, 512 38); half as many again where the rows
+// of a batch take long turns, as T is the longest one's (16 x 2 heads x 168 over up to 4096: 47 -> 38).  A split has a fixed cost
 // of some 5 us and its parts' way through memory: none below 256 keys, 128 where a turn takes
 // four waves' tiles (4 x 80 rows over 1000 tokens 19, by 256 keys 23), and none of one tile's rows up
 // to 512 tokens (12 heads x 8 over 300 tokens 7.4, in two splits 9.6).  Where the rows alone fill
@@ -104,13 +105,15 @@ TreePlan tree_plan(const pa_kv_view& kv, int dtype, int B, int N, int H, int T) 
   const long long base = (long long)B * kv.num_heads * p.row_groups;
   const bool one = p.tiles == 1;
   p.waves = one && base >= 64 && base < 512 && keys > 512 ? tree_most_waves(kv.head_dim) : 4;
-  const long long fill = kv.head_dim == 256 || p.waves == 8 ? 256 : 512;
+  const long long fill = kv.head_dim == 256 || p.waves == 8 ? 256 : one || B == 1 ? 512 : 768;
   const long long least = base >= fill ? 2048 : one ? (keys <= 512 ? 512 : 256) : 128;
   const long long want = base >= fill ? keys : fill / base;
   long long per = std::max(least, (keys + want - 1) / want);
   per = (per + kTreeStep - 1) / kTreeStep * kTreeStep;
   p.split_keys = (int)std::min(per, 1LL << 30);
-  p.nsplit = (int)std::min((keys + per - 1) / per, 1024LL);
+  // (a launch has less than 2^32 threads)
+  p.nsplit = (int)std::min({(keys + per - 1) / per, 1024LL, (1LL << 23) / ((long long)B * kv.num_heads)});
+  p.nsplit = std::max(p.nsplit, 1);
   return p;
 }
 
@@ -204,7 +207,8 @@ extern "C" int pa_tree(const pa_kv_view* kv, const pa_kv_scales* scales, const v
   a.acc = static_cast<float*>(workspace);
   a.ml = a.acc + (size_t)B * N * H * p.nsplit * D;
   const hipStream_t st = as_stream(stream);
-  const dim3 grid(B * kv->num_heads, p.nsplit, p.row_groups);
+  const int pairs = B * kv->num_heads;
+  const dim3 grid = p.tiles == 1 ? dim3(pairs, p.nsplit) : dim3(pairs * p.nsplit, p.row_groups);
   hipError_t e = kv->kv_dtype == LLM_F16    ? launch_tree_f16(a, D, p.tiles, grid, st)
                  : kv->kv_dtype == LLM_BF16 ? launch_tree_bf16(a, D, p.tiles, grid, st)
                  : kv->kv_dtype == LLM_I8   ? launch_tree_i8(a, D, p.tiles, grid, st)

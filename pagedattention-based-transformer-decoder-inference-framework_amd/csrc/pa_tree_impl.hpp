@@ -137,10 +137,14 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 8 / WAVES : 1) void pa_tree_
 
   const int lane = lane_id(), g = lane >> 4, c = lane & 15;
   const int w = wave_id_uniform(), kw = w % KW, rw = w / KW;
-  const int pair = blockIdx.x, b = pair / a.kv_heads, kvh = pair - b * a.kv_heads;
-  const int split = blockIdx.y;
+  // Workgroups go round the XCDs.  Staged, a pair's splits lie beside each other, so that a long row's are
+  // dealt out over all of them (16 x 2 pairs of 168 rows, 11 splits 55 -> 38 us); else the pairs do,
+  // which are many (64 x 16 pairs by splits 249 us, by pairs 241).
+  const int pair = STAGED ? blockIdx.x / a.nsplit : blockIdx.x;
+  const int split = STAGED ? blockIdx.x - pair * a.nsplit : blockIdx.y;
+  const int b = pair / a.kv_heads, kvh = pair - b * a.kv_heads;
   const TreeRow tr = tree_row(a, b);
-  const int first = blockIdx.z * 16 * RW * MT, all_rows = tr.n * a.G;
+  const int first = (STAGED ? blockIdx.y : 0) * 16 * RW * MT, all_rows = tr.n * a.G;
   // the wave's tiles: rows row_of(t) .. + 15, of which the row has rows_of(t)
   auto row_of = [&](int t) { return first + 16 * (rw + RW * t); };
   auto rows_of = [&](int t) { return all_rows - row_of(t); };
@@ -303,8 +307,7 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 8 / WAVES : 1) void pa_tree_
   auto queries = [&] {
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
-      const bool ok = c < rows_of(t);
-      const int row = ok ? row_of(t) + c : 0;  // (no row: the first one's place, as zeros)
+      const int row = c < rows_of(t) ? row_of(t) + c : 0;  // (no row: the first one's, not put out)
       tok[t] = row / a.G;
       const int h = kvh * a.G + row - tok[t] * a.G;
       const size_t at = ((size_t)b * a.N + tok[t]) * a.q_stride + (size_t)h * D;
@@ -328,23 +331,20 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 8 / WAVES : 1) void pa_tree_
           }
         }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          if (!ok) x[kk][e] = 0.f;
-          if (a.scale2 < 0.f) x[kk][e] = -x[kk][e];
-          most = fmaxf(most, fabsf(x[kk][e]));
-        }
+        for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(x[kk][e]));
       }
+      float up = a.scale2 < 0.f ? -1.f : 1.f;  // a scale's sign goes with the queries
       if constexpr (KVT != LLM_BF16) {
         int e = 0;
         (void)frexpf(rows_max(most), &e);  // most < 2^e
         e = clamp_int(e, -100, 128);
-        const float up = ldexpf(1.f, 14 - e);
+        up *= ldexpf(1.f, 14 - e);
         qf[t] = fmaxf(qf[t] * ldexpf(1.f, e - 14), 1e-37f);
-#pragma unroll
-        for (int kk = 0; kk < NK; ++kk)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) x[kk][i] *= up;
       }
+#pragma unroll
+      for (int kk = 0; kk < NK; ++kk)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[kk][i] *= up;
 #pragma unroll
       for (int kk = 0; kk < NK; ++kk)
 #pragma unroll
@@ -520,28 +520,6 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 8 / WAVES : 1) void pa_tree_
         m[t] = top[t];
       }
     }
-    // V^T: the 8 keys' dims exchanged to 8 keys of one dim
-    u32x4 vf[ND];
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf)  // keys 2 hf, 2 hf + 1 of the four
-#pragma unroll
-        for (int e = 0; e < NV; ++e) {
-          const uint32_t v0 = x.v[u][2 * hf][e], v1 = x.v[u][2 * hf + 1][e];
-          if constexpr (QUANT) {
-            const uint32_t flip = KVT == LLM_I8 ? 0x80808080u : 0u;
-            const uint32_t lo2 = __builtin_amdgcn_perm(v1, v0, 0x05010400u) ^ flip;
-            const uint32_t hi2 = __builtin_amdgcn_perm(v1, v0, 0x07030602u) ^ flip;
-            vf[4 * e][2 * u + hf] = two_codes<KVT, false>(lo2);
-            vf[4 * e + 1][2 * u + hf] = two_codes<KVT, true>(lo2);
-            vf[4 * e + 2][2 * u + hf] = two_codes<KVT, false>(hi2);
-            vf[4 * e + 3][2 * u + hf] = two_codes<KVT, true>(hi2);
-          } else {
-            vf[2 * e][2 * u + hf] = __builtin_amdgcn_perm(v1, v0, 0x05040100u);
-            vf[2 * e + 1][2 * u + hf] = __builtin_amdgcn_perm(v1, v0, 0x07060302u);
-          }
-        }
     f32x4 vs[MT][2];  // what probabilities are multiplied by
     if constexpr (QUANT) {
 #pragma unroll
@@ -584,12 +562,36 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 8 / WAVES : 1) void pa_tree_
 #pragma unroll
           for (int i = 0; i < NP; ++i) ph[t][i][2 * u + hf] = part[i];
         }
+    // V^T: the 8 keys' dims exchanged to 8 keys of one dim, a register of each at a time.
+    constexpr int DIMS = 4 / ES;
 #pragma unroll
-    for (int dd = 0; dd < ND; ++dd)
+    for (int e = 0; e < NV; ++e) {
+      u32x4 vf[DIMS];
 #pragma unroll
-      for (int t = 0; t < MT; ++t)
+      for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int i = 0; i < NP; ++i) o[t][dd] = Hf::dot(vf[dd], ph[t][i], o[t][dd]);
+        for (int hf = 0; hf < 2; ++hf) {  // keys 2 hf, 2 hf + 1 of the four
+          const uint32_t v0 = x.v[u][2 * hf][e], v1 = x.v[u][2 * hf + 1][e];
+          if constexpr (QUANT) {
+            const uint32_t flip = KVT == LLM_I8 ? 0x80808080u : 0u;
+            const uint32_t lo2 = __builtin_amdgcn_perm(v1, v0, 0x05010400u) ^ flip;
+            const uint32_t hi2 = __builtin_amdgcn_perm(v1, v0, 0x07030602u) ^ flip;
+            vf[0][2 * u + hf] = two_codes<KVT, false>(lo2);
+            vf[1][2 * u + hf] = two_codes<KVT, true>(lo2);
+            vf[2][2 * u + hf] = two_codes<KVT, false>(hi2);
+            vf[3][2 * u + hf] = two_codes<KVT, true>(hi2);
+          } else {
+            vf[0][2 * u + hf] = __builtin_amdgcn_perm(v1, v0, 0x05040100u);
+            vf[1][2 * u + hf] = __builtin_amdgcn_perm(v1, v0, 0x07060302u);
+          }
+        }
+#pragma unroll
+      for (int i = 0; i < NP; ++i)
+#pragma unroll
+        for (int d = 0; d < DIMS; ++d)
+#pragma unroll
+          for (int t = 0; t < MT; ++t) o[t][DIMS * e + d] = Hf::dot(vf[d], ph[t][i], o[t][DIMS * e + d]);
+    }
   };
 
   // Turns; staged, waves without rows, or without a block in the last one, take their part in the loads.
