@@ -129,8 +129,8 @@ def tree(q, cache, contexts, lens, mask, beams, sm_scale):
                 out[b, i, h] = (w[:, None] * v[see]).sum(0)
                 # A score is off by its queries' halves (2^-22 of each product) and an fp32 sum of D
                 # products (D / 2 roundings of 2^-24 on the way and back, taken as D), its exponent by the
-                # roundings of (s - m) in log2 units; e^x by two steps; a probability's halves by 2^-18
-                # (bf16, the coarser) at most, the sums over the keys by len roundings of 2^-24.  For
+                # roundings of (s - m) in log2 units; e^x by two steps; a probability's parts by 2^-18
+                # (two of bf16, the coarsest) at most, the sums over the keys by len roundings of 2^-24.  For
                 # results in bf16 over other pools a probability is one fp16: rounded by half a step, 2^-11.
                 mags = (k[see].abs() * x.abs()).sum(-1).max() * abs(sm_scale)
                 off = float(mags) * (2.0 ** -22 + (D + 4) * 2.0 ** -24) + \
