@@ -425,7 +425,7 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 8 / WAVES : 1) void pa_tree_
           unusable |= !all;
         }
     }
-    // Scores, in a block of code of its own with their maxima: all tiles' products side by side.
+    const bool more = MT > 1 && rows_of(MT - 1) > 0;  // (a second tile without rows is left out)
     f32x4 s[MT][2];
     {
       u32x4 kf[2][NK];
@@ -445,23 +445,25 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 8 / WAVES : 1) void pa_tree_
           }
         }
 #pragma unroll
-      for (int t = 0; t < MT; ++t)
+      for (int t = 0; t < MT; ++t) {
+        if (t > 0 && !more) break;
 #pragma unroll
         for (int u = 0; u < 2; ++u) s[t][u] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int p = 0; p < NQ; ++p)
+        for (int p = 0; p < NQ; ++p)
 #pragma unroll
-        for (int kk = 0; kk < NK; ++kk)
-#pragma unroll
-          for (int t = 0; t < MT; ++t)
+          for (int kk = 0; kk < NK; ++kk)
 #pragma unroll
             for (int u = 0; u < 2; ++u) s[t][u] = Hf::dot(kf[u][kk], q[t][p][kk], s[t][u]);
+      }
     }
     if constexpr (QUANT) {
 #pragma unroll
-      for (int t = 0; t < MT; ++t)
+      for (int t = 0; t < MT; ++t) {
+        if (t > 0 && !more) break;
 #pragma unroll
         for (int u = 0; u < 2; ++u) s[t][u] *= x.ks[u];
+      }
     }
     uint32_t seen[MT];
     if (special) {
@@ -478,6 +480,7 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 8 / WAVES : 1) void pa_tree_
     bool grown = false;
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
+      if (t > 0 && !more) break;
       float most = -INFINITY;
 #pragma unroll
       for (int u = 0; u < 2; ++u)
@@ -540,7 +543,8 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 8 / WAVES : 1) void pa_tree_
     }
     u32x4 ph[MT][NP];
 #pragma unroll
-    for (int t = 0; t < MT; ++t)
+    for (int t = 0; t < MT; ++t) {
+      if (t > 0 && !more) break;
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -562,6 +566,7 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 8 / WAVES : 1) void pa_tree_
 #pragma unroll
           for (int i = 0; i < NP; ++i) ph[t][i][2 * u + hf] = part[i];
         }
+    }
     // V^T: the 8 keys' dims exchanged to 8 keys of one dim, a register of each at a time.
     constexpr int DIMS = 4 / ES;
 #pragma unroll
@@ -586,11 +591,13 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 8 / WAVES : 1) void pa_tree_
           }
         }
 #pragma unroll
-      for (int i = 0; i < NP; ++i)
+      for (int t = 0; t < MT; ++t) {
+        if (t > 0 && !more) break;
 #pragma unroll
-        for (int d = 0; d < DIMS; ++d)
+        for (int i = 0; i < NP; ++i)
 #pragma unroll
-          for (int t = 0; t < MT; ++t) o[t][DIMS * e + d] = Hf::dot(vf[d], ph[t][i], o[t][DIMS * e + d]);
+          for (int d = 0; d < DIMS; ++d) o[t][DIMS * e + d] = Hf::dot(vf[d], ph[t][i], o[t][DIMS * e + d]);
+      }
     }
   };
 
