@@ -9,6 +9,8 @@ namespace llm {
 namespace {
 
 constexpr int kMergeThreads = 256;
+// From this many rows on a wave joins each, four to a workgroup (16 x 168 rows of 128: 8.5 -> 6.1 us); fewer
+// rows would leave CUs empty: a workgroup each, its waves over the splits.
 constexpr int kWaveRows = 2048;
 
 // A row's parts, relative to the largest of their maxima: `LANES` threads a row, D / 4 of which
@@ -81,39 +83,67 @@ struct TreePlan {
   int row_groups, nsplit, split_keys, waves;
 };
 
-// Splits of equal length, as many as fill the card once: two workgroups a CU, one where heads of 256
-// leave registers for one (16 heads x 63 rows over 32768 e4m3 tokens, us: 256 workgroups 61, 512 54,
-// 1024 65; 8 x 16 heads of 256 over 4000 int8 tokens 256 31, 512 38); half as many again where the rows
-// of a batch take long turns, as T is the longest one's (16 x 2 heads x 168 over up to 4096: 47 -> 38).  A split has a fixed cost
-// of some 5 us and its parts' way through memory: none below 256 keys, 128 where a turn takes
-// four waves' tiles (4 x 80 rows over 1000 tokens 19, by 256 keys 23), and none of one tile's rows up
-// to 512 tokens (12 heads x 8 over 300 tokens 7.4, in two splits 9.6).  Where the rows alone fill
-// the card the parts are there against uneven rows: 2048 keys (64 x 16 heads over up to 8192 int8
-// tokens: whole rows 257 us, 4096 keys 245, 2048 233, 1024 240).
-//
-// One tile's rows of 64 to 511 pairs of long rows take workgroups of 8 waves, half as many splits
-// (4 x 16 heads over up to 8192 fp16 tokens 36.6 -> 32.7 us, 16 x 12 of 64 over 2048 int8, 8 tokens
-// each, 19.6 -> 16.4, no merge); others 4 (12 heads over 1200 int8 tokens 11.7, by 8 waves 12.2; 64 x
-// 16 heads over 500 20.2 and 26.2).
+// Splits of one tile's rows: of equal length, as many as fill the card once, two workgroups of 4 waves a CU,
+// one of 8, or where heads of 256 leave registers for one (8 x 16 heads of 256 over 4000 int8
+// tokens, us: 256 workgroups 31, 512 38).  A split has a fixed cost of some 5 us and its parts' way
+// through memory: none below 256 keys, and none up to 512 tokens (12 heads x 8 over 300 tokens 7.4, in two
+// splits 9.6).  Where the rows alone fill the card the parts are there against uneven rows: 2048
+// keys (64 x 16 heads over up to 8192 int8 tokens: whole rows 257, 4096 keys 245, 2048 233, 1024 240).
+// 64 to 511 pairs of long rows take 8 waves, half as many splits (4 x 16 heads over up to 8192 fp16
+// tokens 36.6 -> 32.7, 16 x 12 of 64 over 2048 int8, 8 tokens each, 19.6 -> 16.4, no merge); others 4 (12
+// heads over 1200 int8 tokens 11.7, by 8 waves 12.2; 64 x 16 heads over 500 20.2 and 26.2).
+void plan_one_tile(TreePlan& p, const pa_kv_view& kv, long long base, long long keys) {
+  p.waves = base >= 64 && base < 512 && keys > 512 ? tree_most_waves(kv.head_dim) : 4;
+  const long long fill = kv.head_dim == 256 || p.waves == 8 ? 256 : 512;
+  const long long least = base >= fill ? 2048 : keys <= 512 ? 512 : 256;
+  const long long want = base >= fill ? keys : fill / base;
+  p.split_keys = (int)std::max(least, (keys + want - 1) / want);
+}
+
+// Splits of more tiles, whose turns are long: the length for which one to four rounds of workgroups, or
+// whole rows, are priced least.  In us, as measured: a workgroup 8 and a turn of its KW blocks 2 (1.4 with
+// one tile a wave, 3.5 of heads of 256), 0.65 of it with a CU to itself; two a CU, three of heads of 64 in 8
+// bits; a merge 6, and every part's way through memory.  The rows of a batch of 4 and more are taken to need
+// 0.6 of T's splits.  (us, whole rows | one round | two: 24 x 16 x 40 rows of 64 over up to 418 int8 tokens 18 | 32
+// | 36; 16 x 2 x 168 over 4096 bf16 - | 39 | 38; 26 x 228 of 64 over 13,805 int8 149 | 83 | 60; 16 x 63 over
+// 32768 e4m3 - | 55 | 67; 2 x 16 x 40 over 4800 fp16 - | 24 | 31.)
+void plan_tiles(TreePlan& p, const pa_kv_view& kv, int parts, int B, int N, int H, long long base, long long keys) {
+  const int D = kv.head_dim, mt = tree_wave_tiles(D, parts);
+  const int turn_keys = kTreeKeys * (mt == 2 && p.tiles == 4 ? 2 : 1);
+  const double share = B >= 4 ? 0.6 : 1.0, turn = D == 256 ? 3.5 : mt == 2 ? 2.0 : 1.4;
+  const double slots = D == 256 ? 256 : D == 64 && paged_elem_size(kv.kv_dtype) == 1 ? 768 : 512;
+  const double part = (double)B * N * H * share * (D + 2) * 8 / 3.5e6;
+  double least = 0;
+  for (int rounds = 0; rounds <= 4; ++rounds) {
+    const long long n = rounds ? std::max(1LL, (long long)(rounds * slots / (share * base))) : 1;
+    const long long per = std::max(128LL, ((keys + n - 1) / n + kTreeStep - 1) / kTreeStep * kTreeStep);
+    const long long m = (keys + per - 1) / per;
+    const double groups = m > 1 ? share * base * m : (double)base;
+    const double one = 8 + (double)per / turn_keys * turn * (groups <= 256 ? 0.65 : 1.0);
+    const double cost = std::ceil(groups / slots) * one + (m > 1 ? 6 + part * m : 0);
+    if (rounds && cost >= least) continue;
+    least = cost;
+    p.split_keys = (int)std::min(per, 1LL << 30);
+  }
+}
+
 TreePlan tree_plan(const pa_kv_view& kv, int dtype, int B, int N, int H, int T) {
   TreePlan p;
-  const int rows = N * (H / kv.num_heads);
-  p.tiles = tree_tiles(kv.head_dim, tree_parts(kv.kv_dtype, dtype), rows);
+  const int rows = N * (H / kv.num_heads), parts = tree_parts(kv.kv_dtype, dtype);
+  p.tiles = tree_tiles(kv.head_dim, parts, rows);
   p.row_groups = (rows + 16 * p.tiles - 1) / (16 * p.tiles);
+  p.waves = 4;
   const long long room = (long long)kv.max_tiles * kv.page_size;
   const long long keys = std::max(1LL, std::min((long long)T + N, room));
   const long long base = (long long)B * kv.num_heads * p.row_groups;
-  const bool one = p.tiles == 1;
-  p.waves = one && base >= 64 && base < 512 && keys > 512 ? tree_most_waves(kv.head_dim) : 4;
-  const long long fill = kv.head_dim == 256 || p.waves == 8 ? 256 : one || B == 1 ? 512 : 768;
-  const long long least = base >= fill ? 2048 : one ? (keys <= 512 ? 512 : 256) : 128;
-  const long long want = base >= fill ? keys : fill / base;
-  long long per = std::max(least, (keys + want - 1) / want);
-  per = (per + kTreeStep - 1) / kTreeStep * kTreeStep;
-  p.split_keys = (int)std::min(per, 1LL << 30);
+  if (p.tiles == 1)
+    plan_one_tile(p, kv, base, keys);
+  else
+    plan_tiles(p, kv, parts, B, N, H, base, keys);
+  p.split_keys = (p.split_keys + kTreeStep - 1) / kTreeStep * kTreeStep;
   // (a launch has less than 2^32 threads)
-  p.nsplit = (int)std::min({(keys + per - 1) / per, 1024LL, (1LL << 23) / ((long long)B * kv.num_heads)});
-  p.nsplit = std::max(p.nsplit, 1);
+  const long long most = std::min(1024LL, (1LL << 23) / ((long long)B * kv.num_heads));
+  p.nsplit = (int)std::max(1LL, std::min((keys + p.split_keys - 1) / p.split_keys, most));
   return p;
 }
 
