@@ -270,8 +270,9 @@ int kv_quant_read(const pa_kv_view* kv, const pa_kv_scales* scales, void* k, voi
  * in full all the same.
  * Scores, sums and the output are accumulated in fp32 (subnormal elements of fp16
  * pools count as 0).  The workspace holds the
- * parts of long rows: pa_tree_workspace_bytes, 16-byte aligned, one for each
- * call that may run at the same time. */
+ * parts of long rows: pa_tree_workspace_bytes of the call's own arguments (a
+ * shorter T may take more parts), 16-byte aligned, one for each call that may
+ * run at the same time. */
 size_t pa_tree_workspace_bytes(const pa_kv_view* kv, int B, int N, int H, int T);
 int pa_tree(const pa_kv_view* kv, const pa_kv_scales* scales, const void* q, long long q_stride,
             void* out, long long out_stride, int dtype, const int32_t* beam_ids,
