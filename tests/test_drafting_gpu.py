@@ -248,6 +248,28 @@ def test_long_rows_in_parts(gpu, cache, D):
         check_tree(c, q, contexts, [3, 2, 3, 0], words, mask, T=T)
 
 
+FORMS = [  # beams, B, N, heads, group, D, contexts
+    (4, 16, 2, 4, 1, 128, [700, 30, 513, 1]),  # 64 pairs of long rows
+    (2, 2, 60, 4, 5, 64, [3000, 40]),  # groups of rows, many parts of them
+    (2, 2, 25, 2, 1, 128, [1900, 900]),  # two tiles in parts
+    (1, 1, 1024, 1, 1, 64, [1500]),  # the most tokens
+    (4, 128, 1, 4, 2, 64, [2300, 2047, 100, 2048]),  # pairs that fill the card, in parts
+]
+
+
+@pytest.mark.parametrize("cache,io", [(F16, F32), (BF16, BF16), (I8, F16), (E4M3, F32), (E4M3, BF16)])
+@pytest.mark.parametrize("form", range(len(FORMS)))
+def test_forms(gpu, cache, io, form):
+    """Batches that are split over keys, rows and waves in the different ways, several rows to a beam, the
+    tokens in chains."""
+    beams, B, N, heads, group, D, contexts = FORMS[form]
+    g = torch.Generator().manual_seed(100 + form)
+    c = Cache(cache, beams, heads, D, 16, max(contexts) + N, seed=form)
+    q = (1.5 * torch.randn((B, N, heads * group, D), generator=g)).to(io)
+    ids = [b % beams for b in range(B)]
+    check_tree(c, q, [contexts[i] for i in ids], [N - b % 2 * (N // 3) for b in range(B)], None, None, beams=ids)
+
+
 @pytest.mark.parametrize("cache", [F16, BF16, I8, E4M3])
 def test_masks_and_missing_pages(gpu, cache):
     """Rows that see nothing, trees of several words, pages that are missing under either half of
