@@ -6,7 +6,9 @@
 // chunk (bit 31: in the prompt, below it the times behind the prompt; whole numbers, so that
 // the order of the additions does not count).  A second word holds the last bias entry of the
 // token, as its place in the list + 1.  History and biases are read by every chunk of the row,
-// from L2, kIds loads of a thread at a time: they are what a short chunk waits for.
+// from L2, kIds loads of a thread at a time: they are what a short chunk waits for (256 rows of 50,257
+// bf16 with history 500 and biases, by 1, 2, 4, 8 and 16 at a time: 18.6, 18.0, 18.5, 20.2 and 23.8 us; 64
+// rows of fp32 with history 4096: 13.5, 12.3, 12.0, 11.9 and 12.4).
 #include "common.hpp"
 #include "paged_rows.hpp"
 
@@ -17,7 +19,7 @@ namespace llm {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kIds = 8;
+constexpr int kIds = 4;
 constexpr uint32_t kPrompt = 0x80000000u;
 
 struct AdjustArgs {
@@ -84,8 +86,8 @@ __global__ __launch_bounds__(kThreads) void logits_adjust_kernel(AdjustArgs a) {
       for (int k = 0; k < kIds; ++k) id[k] = i + k * kThreads < len ? ids[i + k * kThreads] : -1;
 #pragma unroll
       for (int k = 0; k < kIds; ++k) {
-        const uint32_t at = (uint32_t)id[k] - (uint32_t)lo;
-        if (at < (uint32_t)n && id[k] >= 0) f(pad + at, i + k * kThreads);
+        const uint32_t at = (uint32_t)id[k] - (uint32_t)lo;  // (lo + n <= 2^30: negative ids lie behind)
+        if (at < (uint32_t)n) f(pad + at, i + k * kThreads);
       }
     }
   };
@@ -162,9 +164,9 @@ hipError_t launch_chunks(const AdjustArgs& a, int rows, hipStream_t st) {
 }
 
 // Two loads a thread where that leaves 1024 workgroups, the lists being read once for more tokens
-// (64 rows of 50,257 fp32 tokens, history 4096: 12.0 us, by one load 13.7, by four 13.2; 336 of
-// 32,768 bf16: 16.0, 16.5, 20.2), one where the rows are few or both lists take LDS from
-// 16-bit rows, whose chunks are twice as long (256 of 50,257 bf16 with biases: 20.3, by two 24.3).
+// (64 rows of 50,257 fp32 tokens, history 4096: 12.0 us, by one load 13.4; 336 of 32,768 bf16
+// 15.6 and 15.7), one where the rows are few (one row of 50,257: 3.1, by two 3.5) or both lists take LDS
+// from 16-bit rows, whose chunks are twice as long (256 of 50,257 bf16 with biases: 18.5, by two 23.0).
 // An empty launch is 2 us of these; the bytes alone are 5.5, 9.6 and 10.8 at the rate of a copy.
 template <typename T>
 hipError_t launch_adjust(const AdjustArgs& a, int rows, hipStream_t st) {
