@@ -100,27 +100,28 @@ void plan_one_tile(TreePlan& p, const pa_kv_view& kv, long long base, long long 
   p.split_keys = (int)std::max(least, (keys + want - 1) / want);
 }
 
-// Splits of more tiles, whose turns are long: the length for which one to four rounds of workgroups, or
+// Splits of more tiles, whose turns are long: the length for which one or two rounds of workgroups, or
 // whole rows, are priced least.  In us, as measured: a workgroup 8 and a turn of its KW blocks 2 (1.4 with
 // one tile a wave, 3.5 of heads of 256), 0.65 of it with a CU to itself; two a CU, three of heads of 64 in 8
-// bits; a merge 6, and every part's way through memory.  The rows of a batch of 4 and more are taken to need
-// 0.6 of T's splits.  (us, whole rows | one round | two: 24 x 16 x 40 rows of 64 over up to 418 int8 tokens 18 | 32
-// | 36; 16 x 2 x 168 over 4096 bf16 - | 39 | 38; 26 x 228 of 64 over 13,805 int8 149 | 83 | 60; 16 x 63 over
-// 32768 e4m3 - | 55 | 67; 2 x 16 x 40 over 4800 fp16 - | 24 | 31.)
+// bits with more than 64 rows; a merge 4.5, and every part's way through memory.  The rows of a batch of
+// 4 and more are taken to need 0.6 of T's splits.  (us, whole rows | one round | two: 24 x 16 x 40 rows of
+// 64 over up to 418 int8 tokens 18 | 32 | 36; 16 x 2 x 168 over 4096 bf16 - | 39 | 38; 26 x 228 of 64 over
+// 13,805 int8 149 | 83 | 60; 16 x 63 over 32768 e4m3 - | 55 | 67; 2 x 16 x 40 over 4800 fp16 - | 24 | 31;
+// 49 x 2 x 36 over 610 e4m3 23.4 | 17.7.)
 void plan_tiles(TreePlan& p, const pa_kv_view& kv, int parts, int B, int N, int H, long long base, long long keys) {
   const int D = kv.head_dim, mt = tree_wave_tiles(D, parts);
   const int turn_keys = kTreeKeys * (mt == 2 && p.tiles == 4 ? 2 : 1);
   const double share = B >= 4 ? 0.6 : 1.0, turn = D == 256 ? 3.5 : mt == 2 ? 2.0 : 1.4;
-  const double slots = D == 256 ? 256 : D == 64 && paged_elem_size(kv.kv_dtype) == 1 ? 768 : 512;
+  const double slots = D == 256 ? 256 : D == 64 && paged_elem_size(kv.kv_dtype) == 1 && p.tiles == 8 ? 768 : 512;
   const double part = (double)B * N * H * share * (D + 2) * 8 / 3.5e6;
   double least = 0;
-  for (int rounds = 0; rounds <= 4; ++rounds) {
+  for (int rounds = 0; rounds <= 2; ++rounds) {
     const long long n = rounds ? std::max(1LL, (long long)(rounds * slots / (share * base))) : 1;
     const long long per = std::max(128LL, ((keys + n - 1) / n + kTreeStep - 1) / kTreeStep * kTreeStep);
     const long long m = (keys + per - 1) / per;
     const double groups = m > 1 ? share * base * m : (double)base;
-    const double one = 8 + (double)per / turn_keys * turn * (groups <= 256 ? 0.65 : 1.0);
-    const double cost = std::ceil(groups / slots) * one + (m > 1 ? 6 + part * m : 0);
+    const double one = 8 + (double)std::min(per, keys) / turn_keys * turn * (groups <= 256 ? 0.65 : 1.0);
+    const double cost = std::ceil(groups / slots) * one + (m > 1 ? 4.5 + part * m : 0);
     if (rounds && cost >= least) continue;
     least = cost;
     p.split_keys = (int)std::min(per, 1LL << 30);
