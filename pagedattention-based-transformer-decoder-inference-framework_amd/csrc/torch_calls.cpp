@@ -171,7 +171,8 @@ py::object tree(const Tensor& q, const Tensor& k_pool, const Tensor& v_pool, con
   const int dev = k_pool.get_device();
   const pa_kv_view view = view_of(k_pool, v_pool, table, dev);
   pa_kv_scales scales{};
-  if (k_scale) scales = scales_of(k_pool, *k_scale, v_scale.value(), dev);
+  value(k_scale.has_value() == v_scale.has_value(), "scales must be (k_scale, v_scale)");
+  if (k_scale) scales = scales_of(k_pool, *k_scale, *v_scale, dev);
   on_device(q, dev, "q");
   value(q.dim() == 4, "q must be [B][N][H][D]");
   const int64_t B = q.size(0), N = q.size(1), H = q.size(2), D = q.size(3);

@@ -649,3 +649,11 @@ def test_python_refusals(gpu):
                 dict(out=x[:1]), dict(history=i32([1]), frequency=x[0])):
         with pytest.raises((TypeError, ValueError)):
             llm_capi.logits_adjust(x, **bad)
+
+
+def test_scales_go_together(gpu):
+    s = Step()
+    q = torch.zeros((s.d.table.shape[0], 1, s.d.table.shape[1], s.d.k.shape[2]), device="cuda")
+    for bad in ((s.d.scales[0], None), (None, s.d.scales[1])):
+        with pytest.raises(ValueError):
+            llm_capi.pa_tree(q, s.d.k, s.d.v, s.d.table, T=1, scales=bad)
