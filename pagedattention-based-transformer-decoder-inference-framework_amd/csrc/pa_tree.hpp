@@ -1,6 +1,6 @@
 // Attention of drafted tokens over a paged cache (pa_tree; its contract is in llm_decoder.h).
 //
-// A workgroup of 4 waves takes rows (tokens x heads of the group) of one key/value head and one
+// A workgroup of 4 waves (or 8: tree_plan) takes rows (tokens x heads of the group) of one key/value head and one
 // split of its keys, in tiles of 16 rows and blocks of 32 keys.  One tile: the waves take its blocks
 // in turn, from memory straight into registers one block ahead.  Up to 4 tiles: two waves of two
 // tiles each take one block, two the next; up to 8: four waves, two tiles each, take the same
@@ -21,9 +21,17 @@
 // scores, a value's scale its probabilities.
 //
 // Precision: queries enter as parts of 16 bits (fp32 ones as two of fp16, three of bf16: 22 and
-// 24 bits; others exactly), probabilities as two, the rest is fp32.  The products drop fp16
-// subnormals, so a row of queries is scaled to 2^14 by a power of two, probabilities by 2^14, and
-// values' scales are taken in units of a power of two above the largest met.
+// 24 bits; others exactly), probabilities as one to three (launch_tree_parts), the rest is fp32.  The
+// products drop fp16 subnormals, so a row of queries is scaled to 2^14 by a power of two, probabilities
+// by 2^11 (they may grow to 2^15), and values' scales are taken in units of a power of two above the
+// largest met.
+//
+// What bounds it: one tile, the memory (64 x 16 heads of 128 over up to 8192 int8 tokens, pages of 2 KB and
+// their scales in any order: 231 us, 5.2 TB/s; with the products left out 225); more tiles, a
+// SIMD's instructions, of which the scores' exponentials and scales are half (16 heads x 63 rows over 32768
+// e4m3 tokens: 54 us, 2.6 TB/s and 310 TFLOP/s; 16 x 2 x 168 rows over up to 4096 bf16: 33 us): tiles of sums,
+// queries and a block fill the registers of two waves a SIMD.  Short rows, a launch and its code (8 rows of
+// 12 heads over 113 tokens: 5.6 us).
 //
 // Keys that a row does not see get the score -infinity.  Their V still meets a probability of 0
 // in the product, and 0 times NaN is NaN: rows of V that nobody sees (behind the row's end, in
