@@ -21,7 +21,7 @@
 // scores, a value's scale its probabilities.
 //
 // Precision: queries enter as parts of 16 bits (fp32 ones as two of fp16, three of bf16: 22 and
-// 24 bits; others exactly), probabilities as one to three (launch_tree_parts), the rest is fp32.  The
+// 24 bits; others exactly), probabilities as two or three (launch_tree_parts), the rest is fp32.  The
 // products drop fp16 subnormals, so a row of queries is scaled to 2^14 by a power of two, probabilities
 // by 2^11 (they may grow to 2^15), and values' scales are taken in units of a power of two above the
 // largest met.
