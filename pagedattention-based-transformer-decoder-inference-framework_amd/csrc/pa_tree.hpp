@@ -22,9 +22,9 @@
 //
 // Precision: queries enter as parts of 16 bits (fp32 ones as two of fp16, three of bf16: 22 and
 // 24 bits; others exactly), probabilities as two or three (launch_tree_parts), the rest is fp32.  The
-// products drop fp16 subnormals, so a row of queries is scaled to 2^14 by a power of two, probabilities
-// by 2^11 (they may grow to 2^15), and values' scales are taken in units of a power of two above the
-// largest met.
+// numbers that the products see are kept away from fp16's ends: a row of queries is scaled to 2^14 by a power
+// of two, probabilities by 2^11 (they may grow to 2^15), and a value's weight, its probability times its
+// scale, is taken in units of a power of two, a row's own, that goes with the largest weight it has met.
 //
 // What bounds it: one tile, the memory (64 x 16 heads of 128 over up to 8192 int8 tokens, pages of 2 KB and
 // their scales in any order: 231 us, 5.2 TB/s; with the products left out 225); more tiles, a
@@ -35,9 +35,9 @@
 //
 // Keys that a row does not see get the score -infinity.  Their V still meets a probability of 0
 // in the product, and 0 times NaN is NaN: rows of V that nobody sees (behind the row's end, in
-// missing pages) are zeroed, and what is not a number in a drafted token's V is taken as 0;
-// if there was any, the rows that see it get their infinities and NaNs in a pass behind the others,
-// from products of ones.
+// missing pages) are zeroed, and what is not a number in a drafted token's V or its scale is
+// taken as 0; if there was any, the rows that see it get their infinities and NaNs in a pass behind the
+// others, from products of ones.
 #pragma once
 
 #include "common.hpp"

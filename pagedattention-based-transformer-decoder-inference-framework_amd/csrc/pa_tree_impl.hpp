@@ -15,9 +15,9 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 // Operands of 16 bits, as the products of one pool type take them.
 template <bool BF>
 struct Half {  // fp16
-  // Probabilities enter times kP; a maximum moves when it grew by more than kGrow (log2 units), so
-  // that they stay below 2^15: what falls below fp16's normal numbers is 2^-25 of the largest.
-  static constexpr float kP = 2048.f;
+  // Probabilities enter times 2^kP; a maximum moves when it grew by more than kGrow (log2 units), so
+  // that they stay below 2^15: fp16's smallest step, 2^-24, is 2^-34 of the row's largest at most.
+  static constexpr int kP = 11;
   static constexpr float kGrow = 4.f;
   static constexpr uint32_t kOne = 0x3c00u;
   static __device__ __forceinline__ f32x4 dot(u32x4 a, u32x4 b, f32x4 c) {
@@ -34,7 +34,7 @@ struct Half {  // fp16
 };
 template <>
 struct Half<true> {  // bf16
-  static constexpr float kP = 1.f;
+  static constexpr int kP = 0;
   static constexpr float kGrow = 8.f;
   static constexpr uint32_t kOne = 0x3f80u;
   static __device__ __forceinline__ f32x4 dot(u32x4 a, u32x4 b, f32x4 c) {
@@ -358,13 +358,27 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 8 / WAVES : 1) void pa_tree_
   };
 
   f32x4 o[MT][ND];
-  float m[MT], top[MT], l[MT];  // what p is relative to, the maximum (m <= top <= m + kGrow), the sum
-  // of the values' scales: a power of two, at least the largest met; what a probability is multiplied by
-  float unit = 0x1p-100f, per_unit = 0x1p100f * Hf::kP;
+  // what p is relative to (a whole number), the maximum (m < top + 1, top <= m + kRise), the sum
+  float m[MT], top[MT], l[MT];
+  // Weights of quantised values are p times the value's scale, which has any size, and differ from row to
+  // row: o is in units of 2^unit, a row's own.  Blocks whose scales are at most twice that take no more than the
+  // comparison (p is at most 2^kRise, so p scale 2^(kQ - unit) at most 2^15).  A row's new maximum weighs
+  // as much as its scale: where the block's scales are within 2^kUnitAhead of each other, the unit is the largest.
+  // Else, and where a scale is above the unit, the row's weights are looked at: the unit is the
+  // largest, and ahead of it to the largest scale by up to 2^kUnitAhead.  So what a row does not see or weigh does
+  // not take the others' bits: half of fp16's smallest step is 2^-28 of the row's largest weight at most.
+  constexpr int kQ = 8, kUnitAhead = 3, kLeastUnit = -110;
+  constexpr int kW = QUANT ? kQ : Hf::kP;  // what weights enter the products times, log2
+  // (rows move on their own, 32 of a wave, so often that this part counts: 16 heads x 63 rows over 32768 e4m3
+  // tokens 63 us; with kRise 4 and kQ 10 70, with every move's weights looked at 72)
+  constexpr float kRise = QUANT ? 6.f : Hf::kGrow;
+  float per_unit[MT];  // 2^(kQ - unit)
+  auto unit_of = [&](int t) { return kQ + 1 - __builtin_amdgcn_frexp_expf(per_unit[t]); };
 #pragma unroll
   for (int t = 0; t < MT; ++t) {
     m[t] = top[t] = kNegSentinel;
     l[t] = 0.f;
+    per_unit[t] = ldexpf(1.f, kQ - kLeastUnit);
 #pragma unroll
     for (int dd = 0; dd < ND; ++dd) o[t][dd] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
@@ -392,7 +406,7 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 8 / WAVES : 1) void pa_tree_
     if (tr.L - key0 < 32) present &= (1u << (tr.L - key0)) - 1u;
     return present;
   };
-  bool unusable = false;  // a drafted token's V has held infinities or NaNs
+  bool unusable = false;  // a drafted token's V or its scale has held infinities or NaNs
 
   auto attend = [&](Block& x, int i) {
     const int key0 = lo + (i * KW + kw) * kTreeKeys;
@@ -423,6 +437,17 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 8 / WAVES : 1) void pa_tree_
                 x.v[u][r][e] = kept;
               }
           unusable |= !all;
+        }
+      if constexpr (QUANT)
+        if (key0 + kTreeKeys > tr.C) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const bool ok = fabsf(x.vs[u][r]) < INFINITY;
+              unusable |= !ok;
+              x.vs[u][r] = ok ? x.vs[u][r] : 0.f;
+            }
         }
     }
     const bool more = MT > 1 && rows_of(MT - 1) > 0;  // (a second tile without rows is left out)
@@ -465,16 +490,15 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 8 / WAVES : 1) void pa_tree_
         for (int u = 0; u < 2; ++u) s[t][u] *= x.ks[u];
       }
     }
-    uint32_t seen[MT];
     if (special) {
 #pragma unroll
       for (int t = 0; t < MT; ++t) {
-        seen[t] = present & visible(tok[t], key0);
+        const uint32_t seen = present & visible(tok[t], key0);
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            if (!(seen[t] >> (16 * u + 4 * g + r) & 1u)) s[t][u][r] = -INFINITY;
+            if (!(seen >> (16 * u + 4 * g + r) & 1u)) s[t][u][r] = -INFINITY;
       }
     }
     bool grown = false;
@@ -487,58 +511,73 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 8 / WAVES : 1) void pa_tree_
 #pragma unroll
         for (int r = 0; r < 4; ++r) most = fmaxf(most, s[t][u][r]);
       top[t] = fmaxf(top[t], rows_max(most) * qf[t]);
-      grown |= top[t] > m[t] + Hf::kGrow;
+      grown |= top[t] > m[t] + kRise;
     }
+    float largest = 0.f;  // scale
     if constexpr (QUANT) {
-      float most = 0.f;
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) most = fmaxf(most, fabsf(x.vs[u][r]));
-      grown |= most > unit;
+        for (int r = 0; r < 4; ++r) largest = fmaxf(largest, fabsf(x.vs[u][r]));
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        if (t > 0 && !more) break;
+        grown |= largest * per_unit[t] > (float)(2 << kQ);
+      }
     }
-    if (__any(grown)) {  // few blocks: sums move to the new maxima, and to the new unit of scales
-      float down = 1.f;
+    if (__any(grown)) {  // few blocks: rows that grew move to their new maximum, and to a new unit
+      bool apart = false;  // the scales are, or one is above the unit of a row that did not grow
+      int of_scales = 0;
       if constexpr (QUANT) {
-        float most = 0.f;
+        float least = largest;
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (fabsf(x.vs[u][r]) < INFINITY) most = fmaxf(most, fabsf(x.vs[u][r]));
-        most = rows_max(most);
-        int e = 0;
-        (void)frexpf(most, &e);  // most < 2^e
-        const float next = most > unit ? ldexpf(1.f, min(e, 126)) : unit;
-        down = unit / next;
-        per_unit = Hf::kP / next;
-        unit = next;
+          for (int r = 0; r < 4; ++r) least = fminf(least, fabsf(x.vs[u][r]));
+        const float all = rows_max(largest);
+        of_scales = all > 0.f ? __builtin_amdgcn_frexp_expf(all) : kLeastUnit;
+        apart = !(least * ldexpf(1.f, kUnitAhead) >= all && all < INFINITY);
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+          if (t > 0 && !more) break;
+          apart |= !(top[t] > m[t] + kRise) && largest * per_unit[t] > (float)(2 << kQ);
+        }
+        apart = __any(apart);
       }
 #pragma unroll
       for (int t = 0; t < MT; ++t) {
-        const float corr = __builtin_amdgcn_exp2f(m[t] - top[t]);
+        if (t > 0 && !more) break;
+        const bool moves = top[t] > m[t] + kRise;
+        const float next = moves ? ceilf(top[t]) : m[t];
+        const int rise = (int)fmaxf(m[t] - next, -1000.f);  // (<= 0; from the sentinel far below)
+        const float corr = ldexpf(1.f, rise);
         l[t] *= corr;
+        m[t] = next;
+        float down = corr;
+        if constexpr (QUANT) {
+          const int was = unit_of(t) + rise;
+          int to = moves ? max(was, of_scales) : was;
+          if (apart) {
+            float weight = kLeastUnit, scale = kLeastUnit;  // log2, rounded up
 #pragma unroll
-        for (int dd = 0; dd < ND; ++dd) o[t][dd] *= corr * down;
-        m[t] = top[t];
-      }
-    }
-    f32x4 vs[MT][2];  // what probabilities are multiplied by
-    if constexpr (QUANT) {
+            for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        x.vs[u] *= per_unit;
+              for (int r = 0; r < 4; ++r) {
+                const float f = fabsf(x.vs[u][r]), e = __builtin_amdgcn_frexp_expf(f);
+                if (!(f > 0.f && f < INFINITY && s[t][u][r] > -INFINITY)) continue;
+                weight = fmaxf(weight, fmaf(s[t][u][r], qf[t], -m[t]) + e);
+                scale = fmaxf(scale, e);
+                asm volatile("" : "+v"(weight), "+v"(scale));  // (one after the other: the registers are full)
+              }
+            const int of_weight = (int)ceilf(rows_max(weight)), of_scale = (int)rows_max(scale);
+            to = max(was, max(of_weight, min(of_scale, of_weight + kUnitAhead)));
+          }
+          to = max(to, kLeastUnit);
+          down = ldexpf(1.f, was - to);
+          per_unit[t] = ldexpf(1.f, kQ - to);
+        }
 #pragma unroll
-        for (int t = 0; t < MT; ++t) vs[t][u] = x.vs[u];
-      }
-      if (special) {  // (the scale of what is not seen may be NaN)
-#pragma unroll
-        for (int t = 0; t < MT; ++t)
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (!(seen[t] >> (16 * u + 4 * g + r) & 1u)) vs[t][u][r] = 0.f;
+        for (int dd = 0; dd < ND; ++dd) o[t][dd] *= down;
       }
     }
     u32x4 ph[MT][NP];
@@ -556,9 +595,9 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 8 / WAVES : 1) void pa_tree_
             p[e] = __builtin_amdgcn_exp2f(fmaf(s[t][u][r], qf[t], -m[t]));
             l[t] += p[e];
             if constexpr (QUANT) {
-              p[e] *= vs[t][u][r];
-            } else if constexpr (Hf::kP != 1.f) {
-              p[e] *= Hf::kP;
+              p[e] = p[e] * per_unit[t] * x.vs[u][r];  // (in this order: the first product is a number)
+            } else if constexpr (kW != 0) {
+              p[e] *= ldexpf(1.f, kW);
             }
           }
           uint32_t part[NP];
@@ -662,8 +701,7 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 8 / WAVES : 1) void pa_tree_
       }
     }
   }
-  if constexpr (KVT != LLM_I8)
-    if (__any(unusable)) {
+  if (__any(unusable)) {
       // The rows that see them get what the products left out: sums of ones count them.
       for (int i = max((tr.C - lo) / (KW * kTreeKeys) - 1, 0); i < mine; ++i) {
         const int key0 = lo + (i * KW + kw) * kTreeKeys;
@@ -692,10 +730,22 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 8 / WAVES : 1) void pa_tree_
               if (!(present >> (16 * u + key) & 1u)) continue;
               const uint8_t* at = a.v_pool + lane64(at_pool, u) + (uint32_t)(key * ROWB + (c * ND + dd) * ES);
               const uint32_t x = ES == 1 ? *at : *reinterpret_cast<const uint16_t*>(at);
-              constexpr uint32_t kInf = Unusable<KVT>::kInf, kSign = ES == 1 ? 0x80u : 0x8000u;
-              const bool bad = (x & kInf) == kInf, nan = ES == 1 ? bad : (x & (kSign - 1u)) > kInf;
-              if (bad && (nan || !(x & kSign))) plus[e] |= Hf::kOne << 16 * s;
-              if (bad && (nan || (x & kSign))) minus[e] |= Hf::kOne << 16 * s;
+              constexpr uint32_t kSign = ES == 1 ? 0x80u : 0x8000u;
+              bool bad = false, nan = false, minus_of = (x & kSign) != 0;
+              if constexpr (KVT != LLM_I8) {
+                constexpr uint32_t kInf = Unusable<KVT>::kInf;
+                bad = (x & kInf) == kInf, nan = ES == 1 ? bad : (x & (kSign - 1u)) > kInf;
+              }
+              if constexpr (QUANT)
+                if (a.v_scale) {
+                  const float f = *reinterpret_cast<const float*>(reinterpret_cast<const uint8_t*>(a.v_scale) +
+                                                                  lane64(at_scale, u) + 4 * key);
+                  bad |= !(fabsf(f) < INFINITY);
+                  nan |= f != f || !(KVT == LLM_I8 ? x : x & (kSign - 1u));  // (infinity times 0)
+                  minus_of ^= f < 0.f;
+                }
+              if (bad && (nan || !minus_of)) plus[e] |= Hf::kOne << 16 * s;
+              if (bad && (nan || minus_of)) minus[e] |= Hf::kOne << 16 * s;
             }
           }
           const f32x4 none = {0.f, 0.f, 0.f, 0.f};
@@ -717,7 +767,7 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 8 / WAVES : 1) void pa_tree_
   for (int t = 0; t < MT; ++t) {
     const float back = __builtin_amdgcn_exp2f(m[t] - top[t]);
     const float sum = add(with_lane32(add(with_lane16(l[t] * back))));
-    const float f = back * (QUANT ? unit / Hf::kP : 1.f / Hf::kP);
+    const float f = ldexpf(back, (QUANT ? unit_of(t) : 0) - kW);
     if (t) __syncthreads();  // the tiles before are read
 #pragma unroll
     for (int r = 0; r < 4; ++r)

@@ -3,11 +3,13 @@ whose value scales or scores lie far from the others'.
 
 Tolerances.  With w the weights of a row's keys (they add up to 1) and v their values, a result is off
 by at most
-    sum(w |v|) (2 off + 2^-18 + (keys + 16) 2^-24) + 2^-34 max(w |scale|) sum |code|
+    sum(w |v|) (2 off + 2^-18 + (keys + 16) 2^-24) + 2^-28 max(w |scale|) sum |code|
 and half a step of its type: `off` is the error of a score (queries in two halves, 2^-22 of each product,
 D sums of 2^-24, the exponent's roundings), counted twice for a key and the sum; a probability enters
-the products in two halves of 11 bits and its rescalings (2^-18 together), or with the smallest step of fp16 next
-to a row's largest; sums of fp32 are off by 2^-24 a key.  Where values have no scales, scale = 1."""
+the products in two halves of 11 bits and its rescalings (2^-18 together), and is off by half of fp16's
+smallest step, 2^-25, besides: weights enter times 2^8 in units of at most 2^5 times the row's largest one
+(a power of two from the product of two numbers rounded up to theirs, 2^2, and 2^3 ahead of it), so
+2^-25 2^-8 2^5 = 2^-28 of it; sums of fp32 are off by 2^-24 a key.  Where values have no scales, scale = 1."""
 import pytest
 import torch
 
@@ -54,7 +56,7 @@ def attention(q, c, contexts, mask, sm_scale):
             off = (x.abs() @ k[see].abs().T.contiguous()).amax(1) * abs(sm_scale) * (2.0 ** -22 + (D + 4) * 2.0 ** -24) \
                 + 4 * (s.abs().amax(1) + 1) * 2.0 ** -23 + 2.0 ** -22
             share = 2 * off + 2.0 ** -18 + (int(see.sum()) + 16) * 2.0 ** -24
-            tail = 2.0 ** -34 * (w * scale[see].abs()).amax(1)
+            tail = 2.0 ** -28 * (w * scale[see].abs()).amax(1)
             room[b, i] = share[:, None] * (w @ v[see].abs()) + tail[:, None] * code[see].abs().sum(0)
     return out, room
 
@@ -96,3 +98,75 @@ def test_values_that_nearly_cancel(gpu, cache, io, N, H, D):
         put(c, "v", 0, pos, torch.zeros(D))
     q = (1.5 * torch.randn((1, N, H, D), generator=g)).to(io)
     check(c, q, [C])
+
+
+def positive_rows(N, H, D, io, g):
+    """Queries whose every element is positive, so that a key of one sign scores low for all of them."""
+    return (0.5 + torch.rand((1, N, H, D), generator=g)).to(io)
+
+
+@pytest.mark.parametrize("cache", [I8, E4M3])
+@pytest.mark.parametrize("io", [F32, BF16])
+@pytest.mark.parametrize("N,H", ROWS)
+@pytest.mark.parametrize("far", [14, 25, 40, 80])
+def test_unseen_drafts_of_large_scales(gpu, cache, io, N, H, far):
+    """A drafted token whose value scale is 2^far times the others': rows that do not see it have
+    their own values, rows that see it its."""
+    g = torch.Generator().manual_seed(far + N)
+    C = 77
+    c = Cache(cache, 1, 1, 64, 16, C + N, seed=N)
+    c.scales[1][c.slot(0, 0, C + 1)] *= 2.0 ** far
+    q = (1.5 * torch.randn((1, N, H, 64), generator=g)).to(io)
+    mask = torch.eye(N, dtype=torch.bool)[None].clone()
+    mask[:, N - 1, 1] = True
+    words = torch.zeros((1, N, -(-N // 32) * 32), dtype=torch.int64)
+    words[..., :N] = mask
+    words = (words.view(1, N, -1, 32) << torch.arange(32)).sum(-1)
+    words = torch.where(words >= 1 << 31, words - (1 << 32), words).to(torch.int32)
+    check(c, q, [C], words, mask)
+    check(c, q, [C], words, mask, T=4000)
+
+
+@pytest.mark.parametrize("cache", [I8, E4M3])
+@pytest.mark.parametrize("io", [F32, BF16])
+@pytest.mark.parametrize("N,H", [(1, 1)] + ROWS)
+@pytest.mark.parametrize("far", [14, 25, 40, 80])
+@pytest.mark.parametrize("pos", [0, 50, 158])
+def test_keys_of_no_weight_and_large_scale(gpu, cache, io, N, H, far, pos):
+    """A committed key whose score is some 70 below the others' and whose value scale 2^far times theirs,
+    ahead of them, among them and behind them."""
+    g = torch.Generator().manual_seed(far + N)
+    C = 160
+    c = Cache(cache, 1, 1, 64, 16, C + N, seed=N)
+    q = positive_rows(N, H, 64, io, g)
+    put(c, "k", 0, pos, torch.full((64,), -96.0), 70 * 8 / (64 * 96.0))
+    c.scales[1][c.slot(0, 0, pos)] *= 2.0 ** far
+    check(c, q, [C])
+
+
+@pytest.mark.parametrize("cache", [I8, E4M3])
+@pytest.mark.parametrize("N,H", [(1, 1)] + ROWS)
+@pytest.mark.parametrize("up", [0.3, -0.3, 3.0])
+def test_scores_that_rise_and_fall(gpu, cache, N, H, up):
+    """Scores that go up (or down) by a step from key to key, over scales that go the other way."""
+    g = torch.Generator().manual_seed(N)
+    C = 320
+    c = Cache(cache, 1, 1, 64, 16, C + N, seed=N)
+    q = positive_rows(N, H, 64, F32, g)
+    for t in range(C + N):
+        put(c, "k", 0, t, torch.full((64,), 96.0), (t - C / 2) * up * 8 / (64 * 96.0))
+        c.scales[1][c.slot(0, 0, t)] *= 2.0 ** (-(t - C / 2) * up / 4)
+    check(c, q, [C])
+
+
+@pytest.mark.parametrize("cache", [I8, E4M3])
+@pytest.mark.parametrize("size", [-140, -120, -100, 100, 118])
+def test_scales_of_any_size(gpu, cache, size):
+    """Value scales from fp32's subnormal numbers to its largest ones, one of no weight among them."""
+    c = Cache(cache, 1, 1, 64, 16, 300, seed=7)
+    q = positive_rows(3, 2, 64, F32, torch.Generator().manual_seed(1))
+    c.scales[1] = (c.scales[1].double() * 2.0 ** size).float()
+    check(c, q, [290])
+    c.scales[1][c.slot(0, 0, 40)] = 0.0
+    c.scales[1][c.slot(0, 0, 41)] *= -1.0
+    check(c, q, [290])
