@@ -16,15 +16,15 @@
 // bytes among its own registers (v_perm), so V^T needs no LDS.  Tile dd of O^T then has rows
 // m = c for the dims c D/16 + dd: lane (g, c) ends with dims 4 g D/16 .. (4 g + 4) D/16 of row c.
 //
-// 8-bit codes become fp16 on the way into the products, exactly (int8: 0x6400 | code ^ 0x80 is
-// the fp16 number 1152 + code; e4m3: one conversion for two).  A key's scale multiplies its
+// 8-bit codes become 16 bits on the way into the products, exactly: keys' fp16 (int8: 0x6400 | code ^ 0x80 is
+// the fp16 number 1152 + code; e4m3: one conversion for two), values' bf16.  A key's scale multiplies its
 // scores, a value's scale its probabilities.
 //
 // Precision: queries enter as parts of 16 bits (fp32 ones as two of fp16, three of bf16: 22 and
-// 24 bits; others exactly), probabilities as two or three (launch_tree_parts), the rest is fp32.  The
-// numbers that the products see are kept away from fp16's ends: a row of queries is scaled to 2^14 by a power
-// of two, probabilities by 2^11 (they may grow to 2^15), and a value's weight, its probability times its
-// scale, is taken in units of a power of two, a row's own, that goes with the largest weight it has met.
+// 24 bits; others exactly), probabilities as two or three (launch_tree_parts), the rest is fp32.  The products
+// keep subnormal numbers.  fp16 ones are kept away from its ends: a row of queries is scaled to 2^14 by a power of
+// two, probabilities by 2^11 (they may grow to 2^15).  Quantised values' weights, probabilities times scales,
+// are bf16, which has fp32's range.
 //
 // What bounds it: one tile, the memory (64 x 16 heads of 128 over up to 8192 int8 tokens, pages of 2 KB and
 // their scales in any order: 231 us, 5.2 TB/s; with the products left out 225); more tiles, a

@@ -15,9 +15,9 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 // Operands of 16 bits, as the products of one pool type take them.
 template <bool BF>
 struct Half {  // fp16
-  // Probabilities enter times 2^kP; a maximum moves when it grew by more than kGrow (log2 units), so
-  // that they stay below 2^15: fp16's smallest step, 2^-24, is 2^-34 of the row's largest at most.
-  static constexpr int kP = 11;
+  // Probabilities enter times kP; a maximum moves when it grew by more than kGrow (log2 units), so
+  // that they stay below 2^15: half of fp16's smallest step, 2^-25, is 2^-35 of the row's largest at most.
+  static constexpr float kP = 2048.f;
   static constexpr float kGrow = 4.f;
   static constexpr uint32_t kOne = 0x3c00u;
   static __device__ __forceinline__ f32x4 dot(u32x4 a, u32x4 b, f32x4 c) {
@@ -34,7 +34,7 @@ struct Half {  // fp16
 };
 template <>
 struct Half<true> {  // bf16
-  static constexpr int kP = 0;
+  static constexpr float kP = 1.f;
   static constexpr float kGrow = 8.f;
   static constexpr uint32_t kOne = 0x3f80u;
   static __device__ __forceinline__ f32x4 dot(u32x4 a, u32x4 b, f32x4 c) {
@@ -73,6 +73,15 @@ __device__ __forceinline__ uint32_t two_codes(uint32_t w) {
   } else {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, HIGH));
   }
+}
+
+// One byte of two registers each, as two halves of bf16 (exact: codes have 8 bits at most).
+__device__ __forceinline__ uint32_t two_bytes(uint32_t a, uint32_t b, int byte) {
+  return Half<true>::pair((float)(int8_t)(a >> 8 * byte), (float)(int8_t)(b >> 8 * byte));
+}
+template <bool HIGH>
+__device__ __forceinline__ uint32_t two_e4m3(uint32_t w) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, HIGH));
 }
 
 template <int KVT>
@@ -114,7 +123,8 @@ template <int KVT, int D, int NQ, int NP, int WAVES, int KW, int MT>
 __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 8 / WAVES : 1) void pa_tree_kernel(TreeArgs a) {
   constexpr bool QUANT = Raw<KVT>::QUANT;
   constexpr int ES = Raw<KVT>::ES, ROWB = D * ES;
-  using Hf = Half<KVT == LLM_BF16>;
+  using Hf = Half<KVT == LLM_BF16>;           // of scores' products
+  using Pf = Half<KVT == LLM_BF16 || QUANT>;  // of values'
   constexpr int NK = D / 32;          // steps of 32 dims of q.k
   constexpr int NKL = ROWB / 64;      // 16-byte loads of a key tile
   constexpr int ND = D / 16;          // tiles of the output, dims of a lane's keys
@@ -358,27 +368,21 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 8 / WAVES : 1) void pa_tree_
   };
 
   f32x4 o[MT][ND];
-  // what p is relative to (a whole number), the maximum (m < top + 1, top <= m + kRise), the sum
+  // what p is relative to (a whole number), the maximum (m + kLift < top + 1, top <= m + kRise), the sum
   float m[MT], top[MT], l[MT];
-  // Weights of quantised values are p times the value's scale, which has any size, and differ from row to
-  // row: o is in units of 2^unit, a row's own.  Blocks whose scales are at most twice that take no more than the
-  // comparison (p is at most 2^kRise, so p scale 2^(kQ - unit) at most 2^15).  A row's new maximum weighs
-  // as much as its scale: where the block's scales are within 2^kUnitAhead of each other, the unit is the largest.
-  // Else, and where a scale is above the unit, the row's weights are looked at: the unit is the
-  // largest, and ahead of it to the largest scale by up to 2^kUnitAhead.  So what a row does not see or weigh does
-  // not take the others' bits: half of fp16's smallest step is 2^-28 of the row's largest weight at most.
-  constexpr int kQ = 8, kUnitAhead = 3, kLeastUnit = -110;
-  constexpr int kW = QUANT ? kQ : Hf::kP;  // what weights enter the products times, log2
-  // (rows move on their own, 32 of a wave, so often that this part counts: 16 heads x 63 rows over 32768 e4m3
-  // tokens 63 us; with kRise 4 and kQ 10 70, with every move's weights looked at 72)
-  constexpr float kRise = QUANT ? 6.f : Hf::kGrow;
-  float per_unit[MT];  // 2^(kQ - unit)
-  auto unit_of = [&](int t) { return kQ + 1 - __builtin_amdgcn_frexp_expf(per_unit[t]); };
+  // Weights of quantised values, p times the value's scale, enter the products in bf16 and so have all of fp32's
+  // range: scales have any size, and what a row does not see or weigh must not take the others' bits.  p is 2^kLift
+  // of a probability, so that scales up to kHuge leave fp32's normal numbers at neither end.  At a larger one
+  // the row's weights are looked at; a row with one above 2^100 is in units of its own from then on.
+  constexpr int kLift = QUANT ? 40 : 0;
+  constexpr float kRise = (float)kLift + Pf::kGrow, kHuge = 0x1p50f;
+  float per_unit[MT];    // <= 1
+  bool units = false;    // one of them is not 1
 #pragma unroll
   for (int t = 0; t < MT; ++t) {
     m[t] = top[t] = kNegSentinel;
     l[t] = 0.f;
-    per_unit[t] = ldexpf(1.f, kQ - kLeastUnit);
+    per_unit[t] = 1.f;
 #pragma unroll
     for (int dd = 0; dd < ND; ++dd) o[t][dd] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
@@ -519,65 +523,59 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 8 / WAVES : 1) void pa_tree_
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int r = 0; r < 4; ++r) largest = fmaxf(largest, fabsf(x.vs[u][r]));
-#pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        if (t > 0 && !more) break;
-        grown |= largest * per_unit[t] > (float)(2 << kQ);
-      }
+      grown |= largest > kHuge;
     }
-    if (__any(grown)) {  // few blocks: rows that grew move to their new maximum, and to a new unit
-      bool apart = false;  // the scales are, or one is above the unit of a row that did not grow
-      int of_scales = 0;
-      if constexpr (QUANT) {
-        float least = largest;
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) least = fminf(least, fabsf(x.vs[u][r]));
-        const float all = rows_max(largest);
-        of_scales = all > 0.f ? __builtin_amdgcn_frexp_expf(all) : kLeastUnit;
-        apart = !(least * ldexpf(1.f, kUnitAhead) >= all && all < INFINITY);
-#pragma unroll
-        for (int t = 0; t < MT; ++t) {
-          if (t > 0 && !more) break;
-          apart |= !(top[t] > m[t] + kRise) && largest * per_unit[t] > (float)(2 << kQ);
-        }
-        apart = __any(apart);
-      }
+    if (__any(grown)) {  // few blocks: sums move to the new maxima
+      const bool huge = QUANT && (units || __any(largest > kHuge));
 #pragma unroll
       for (int t = 0; t < MT; ++t) {
         if (t > 0 && !more) break;
-        const bool moves = top[t] > m[t] + kRise;
-        const float next = moves ? ceilf(top[t]) : m[t];
+        const float next = ceilf(top[t]) - (float)kLift;
         const int rise = (int)fmaxf(m[t] - next, -1000.f);  // (<= 0; from the sentinel far below)
         const float corr = ldexpf(1.f, rise);
         l[t] *= corr;
         m[t] = next;
         float down = corr;
-        if constexpr (QUANT) {
-          const int was = unit_of(t) + rise;
-          int to = moves ? max(was, of_scales) : was;
-          if (apart) {
-            float weight = kLeastUnit, scale = kLeastUnit;  // log2, rounded up
+        if constexpr (QUANT)
+          if (huge) {
+            float weight = -1000.f;  // log2, rounded up
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
               for (int r = 0; r < 4; ++r) {
-                const float f = fabsf(x.vs[u][r]), e = __builtin_amdgcn_frexp_expf(f);
-                if (!(f > 0.f && f < INFINITY && s[t][u][r] > -INFINITY)) continue;
-                weight = fmaxf(weight, fmaf(s[t][u][r], qf[t], -m[t]) + e);
-                scale = fmaxf(scale, e);
-                asm volatile("" : "+v"(weight), "+v"(scale));  // (one after the other: the registers are full)
+                const float f = fabsf(x.vs[u][r]);
+                if (f > 0.f && f < INFINITY)
+                  weight = fmaxf(weight, fmaf(s[t][u][r], qf[t], -m[t]) + __builtin_amdgcn_frexp_expf(f));
+                asm volatile("" : "+v"(weight));  // (one after the other: the registers are full)
               }
-            const int of_weight = (int)ceilf(rows_max(weight)), of_scale = (int)rows_max(scale);
-            to = max(was, max(of_weight, min(of_scale, of_weight + kUnitAhead)));
+            const int was = 1 - __builtin_amdgcn_frexp_expf(per_unit[t]) + rise;
+            const int to = max(max(was, 0), (int)ceilf(rows_max(weight)) - 100);
+            down = ldexpf(1.f, was - to);
+            per_unit[t] = ldexpf(1.f, -to);
           }
-          to = max(to, kLeastUnit);
-          down = ldexpf(1.f, was - to);
-          per_unit[t] = ldexpf(1.f, kQ - to);
-        }
 #pragma unroll
         for (int dd = 0; dd < ND; ++dd) o[t][dd] *= down;
+      }
+      if (huge) units = __any(per_unit[0] != 1.f || per_unit[MT - 1] != 1.f);
+    }
+    f32x4 p[MT][2];
+    if constexpr (QUANT) {
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        if (t > 0 && !more) break;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            p[t][u][r] = __builtin_amdgcn_exp2f(fmaf(s[t][u][r], qf[t], -m[t]));
+            l[t] += p[t][u][r];
+          }
+      }
+      if (units) {  // (ahead of the scale, whose product with a probability may be no fp32 number)
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) p[t][u] *= per_unit[t];
       }
     }
     u32x4 ph[MT][NP];
@@ -588,20 +586,20 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 8 / WAVES : 1) void pa_tree_
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
-          float p[2];
+          float w[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const int r = 2 * hf + e;
-            p[e] = __builtin_amdgcn_exp2f(fmaf(s[t][u][r], qf[t], -m[t]));
-            l[t] += p[e];
             if constexpr (QUANT) {
-              p[e] = p[e] * per_unit[t] * x.vs[u][r];  // (in this order: the first product is a number)
-            } else if constexpr (kW != 0) {
-              p[e] *= ldexpf(1.f, kW);
+              w[e] = p[t][u][r] * x.vs[u][r];
+            } else {
+              w[e] = __builtin_amdgcn_exp2f(fmaf(s[t][u][r], qf[t], -m[t]));
+              l[t] += w[e];
+              w[e] *= Pf::kP;
             }
           }
           uint32_t part[NP];
-          split_parts<Hf, NP>(p[0], p[1], part);
+          split_parts<Pf, NP>(w[0], w[1], part);
 #pragma unroll
           for (int i = 0; i < NP; ++i) ph[t][i][2 * u + hf] = part[i];
         }
@@ -616,14 +614,16 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 8 / WAVES : 1) void pa_tree_
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {  // keys 2 hf, 2 hf + 1 of the four
           const uint32_t v0 = x.v[u][2 * hf][e], v1 = x.v[u][2 * hf + 1][e];
-          if constexpr (QUANT) {
-            const uint32_t flip = KVT == LLM_I8 ? 0x80808080u : 0u;
-            const uint32_t lo2 = __builtin_amdgcn_perm(v1, v0, 0x05010400u) ^ flip;
-            const uint32_t hi2 = __builtin_amdgcn_perm(v1, v0, 0x07030602u) ^ flip;
-            vf[0][2 * u + hf] = two_codes<KVT, false>(lo2);
-            vf[1][2 * u + hf] = two_codes<KVT, true>(lo2);
-            vf[2][2 * u + hf] = two_codes<KVT, false>(hi2);
-            vf[3][2 * u + hf] = two_codes<KVT, true>(hi2);
+          if constexpr (KVT == LLM_I8) {
+#pragma unroll
+            for (int d = 0; d < 4; ++d) vf[d][2 * u + hf] = two_bytes(v0, v1, d);
+          } else if constexpr (KVT == LLM_E4M3) {
+            const uint32_t lo2 = __builtin_amdgcn_perm(v1, v0, 0x05010400u);
+            const uint32_t hi2 = __builtin_amdgcn_perm(v1, v0, 0x07030602u);
+            vf[0][2 * u + hf] = two_e4m3<false>(lo2);
+            vf[1][2 * u + hf] = two_e4m3<true>(lo2);
+            vf[2][2 * u + hf] = two_e4m3<false>(hi2);
+            vf[3][2 * u + hf] = two_e4m3<true>(hi2);
           } else {
             vf[0][2 * u + hf] = __builtin_amdgcn_perm(v1, v0, 0x05040100u);
             vf[1][2 * u + hf] = __builtin_amdgcn_perm(v1, v0, 0x07060302u);
@@ -635,7 +635,7 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 8 / WAVES : 1) void pa_tree_
 #pragma unroll
         for (int i = 0; i < NP; ++i)
 #pragma unroll
-          for (int d = 0; d < DIMS; ++d) o[t][DIMS * e + d] = Hf::dot(vf[d], ph[t][i], o[t][DIMS * e + d]);
+          for (int d = 0; d < DIMS; ++d) o[t][DIMS * e + d] = Pf::dot(vf[d], ph[t][i], o[t][DIMS * e + d]);
       }
     }
   };
@@ -767,7 +767,7 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 8 / WAVES : 1) void pa_tree_
   for (int t = 0; t < MT; ++t) {
     const float back = __builtin_amdgcn_exp2f(m[t] - top[t]);
     const float sum = add(with_lane32(add(with_lane16(l[t] * back))));
-    const float f = ldexpf(back, (QUANT ? unit_of(t) : 0) - kW);
+    const float f = ldexpf(back * (1.f / Pf::kP), 1 - __builtin_amdgcn_frexp_expf(per_unit[t]));
     if (t) __syncthreads();  // the tiles before are read
 #pragma unroll
     for (int r = 0; r < 4; ++r)
@@ -848,14 +848,15 @@ hipError_t launch_tree_dim(const TreeArgs& a, int D, int tiles, dim3 grid, hipSt
                     : launch_tree_tiles<KVT, 256, NQ, NP>(a, tiles, grid, st);
 }
 
-// Probabilities are two parts, of bf16 for fp32 results three (two are off by 2^-18, four times what fp32
-// sums of the products are).  One of fp16 for results in bf16, whose own rounding is by up to 2^-8, would be
-// off by 2^-11 of every weight, which shows where values cancel: 1e-4 beside a result of 4e-5.  It was
-// 57.5 us where two are 62.8 (16 heads x 63 rows over 32768 e4m3 tokens).
+// Weights are two parts of 11 bits over fp16 pools, of 8 else and then three for fp32 results (two are off
+// by 2^-17, eight times what fp32 sums of the products are).  One of fp16 for results in bf16, whose own
+// rounding is by up to 2^-8, would be off by 2^-11 of every weight, which shows where values cancel: 1e-4
+// beside a result of 4e-5.  fp16 pools' parts drop what is below 2^-35 of the row's largest weight; a third
+// one in bf16, values too, would keep it (fp32 results, 26 x 4 x 228 rows of 64 over up to 8000 tokens: 161 -> 202
+// us; one row of 128 32.5 -> 34).
 template <int KVT>
 hipError_t launch_tree_parts(const TreeArgs& a, int D, int tiles, dim3 grid, hipStream_t st) {
-  constexpr bool BF = KVT == LLM_BF16;
-  return a.dtype == LLM_F32   ? launch_tree_dim<KVT, tree_parts(KVT, LLM_F32), BF ? 3 : 2>(a, D, tiles, grid, st)
+  return a.dtype == LLM_F32   ? launch_tree_dim<KVT, tree_parts(KVT, LLM_F32), KVT == LLM_F16 ? 2 : 3>(a, D, tiles, grid, st)
          : a.dtype == LLM_F16 ? launch_tree_dim<KVT, tree_parts(KVT, LLM_F16), 2>(a, D, tiles, grid, st)
                               : launch_tree_dim<KVT, tree_parts(KVT, LLM_BF16), 2>(a, D, tiles, grid, st);
 }

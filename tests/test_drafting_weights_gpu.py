@@ -3,18 +3,18 @@ whose value scales or scores lie far from the others'.
 
 Tolerances.  With w the weights of a row's keys (they add up to 1) and v their values, a result is off
 by at most
-    sum(w |v|) (2 off + 2^-18 + (keys + 16) 2^-24) + 2^-28 max(w |scale|) sum |code|
+    sum(w |v|) (2 off + 2^-17 + (keys + 16) 2^-24)
 and half a step of its type: `off` is the error of a score (queries in two halves, 2^-22 of each product,
-D sums of 2^-24, the exponent's roundings), counted twice for a key and the sum; a probability enters
-the products in two halves of 11 bits and its rescalings (2^-18 together), and is off by half of fp16's
-smallest step, 2^-25, besides: weights enter times 2^8 in units of at most 2^5 times the row's largest one
-(a power of two from the product of two numbers rounded up to theirs, 2^2, and 2^3 ahead of it), so
-2^-25 2^-8 2^5 = 2^-28 of it; sums of fp32 are off by 2^-24 a key.  Where values have no scales, scale = 1."""
+D sums of 2^-24, the exponent's roundings), counted twice for a key and the sum; a weight enters the products in
+two parts of 8 bits at least (half a step of the first is 2^-9 of it, of the second 2^-9 of what is left, 2^-18)
+and its roundings ahead of them, 2^-18 in all; sums of fp32 are off by 2^-24 a key.  Over fp16 pages the parts
+are fp16: half of the smallest step, 2^-25, of probabilities times 2^11, relative to at most twice the
+row's largest, is 2^-35 of it, so 2^-35 max(w) sum |v| more."""
 import pytest
 import torch
 
 import llm_capi
-from _drafting import Cache, bits, close
+from _drafting import Cache, close
 
 pytestmark = pytest.mark.gpu
 I8, E4M3 = torch.int8, torch.float8_e4m3fn
@@ -29,7 +29,7 @@ def put(c, name, b, pos, codes, scale=None):
     """Codes (and the scale) of one token of head 0."""
     at = c.slot(b, 0, pos)
     getattr(c, name)[at] = codes.to(c.dtype)
-    if scale is not None:
+    if scale is not None and c.scales is not None:
         c.scales["kv".index(name)][at] = scale
 
 
@@ -41,9 +41,6 @@ def attention(q, c, contexts, mask, sm_scale):
         L = contexts[b] + N
         k, ok = c.held("k", b, 0, L)
         v, _ = c.held("v", b, 0, L)
-        at = torch.tensor([c.slot(b, 0, t) for t in range(L)])
-        scale = c.scales[1][at[:, 0], at[:, 1]].double() if c.scales is not None else torch.ones(L).double()
-        code = bits(c.v)[at[:, 0], at[:, 1]].view(c.dtype).double()
         j = torch.arange(L) - contexts[b]
         for i in range(N):
             own = torch.arange(N) <= i if mask is None else mask[b, i]
@@ -55,9 +52,10 @@ def attention(q, c, contexts, mask, sm_scale):
             out[b, i] = w @ v[see]
             off = (x.abs() @ k[see].abs().T.contiguous()).amax(1) * abs(sm_scale) * (2.0 ** -22 + (D + 4) * 2.0 ** -24) \
                 + 4 * (s.abs().amax(1) + 1) * 2.0 ** -23 + 2.0 ** -22
-            share = 2 * off + 2.0 ** -18 + (int(see.sum()) + 16) * 2.0 ** -24
-            tail = 2.0 ** -28 * (w * scale[see].abs()).amax(1)
-            room[b, i] = share[:, None] * (w @ v[see].abs()) + tail[:, None] * code[see].abs().sum(0)
+            share = 2 * off + 2.0 ** -17 + (int(see.sum()) + 16) * 2.0 ** -24
+            room[b, i] = share[:, None] * (w @ v[see].abs())
+            if c.dtype == F16:
+                room[b, i] += 2.0 ** -35 * w.amax(1)[:, None] * v[see].abs().sum(0)
     return out, room
 
 
@@ -170,3 +168,32 @@ def test_scales_of_any_size(gpu, cache, size):
     c.scales[1][c.slot(0, 0, 40)] = 0.0
     c.scales[1][c.slot(0, 0, 41)] *= -1.0
     check(c, q, [290])
+
+
+@pytest.mark.parametrize("cache", [F16, BF16, I8, E4M3])
+@pytest.mark.parametrize("io", [F32, F16, BF16])
+@pytest.mark.parametrize("N,H", [(1, 1)] + ROWS)
+@pytest.mark.parametrize("far", [12, 20, 26, 32, 60])
+def test_many_keys_far_below_one_without_value(gpu, cache, io, N, H, far):
+    """A key that has next to all the weight and the value 0: the result is the others', whose weights are 2^-far
+    of its."""
+    C, D = 700, 64
+    c = Cache(cache, 1, 1, D, 16, C + N, seed=far)
+    q = positive_rows(N, H, D, io, torch.Generator().manual_seed(far))
+    low = 0.25 * far / 96 if cache in (I8, E4M3) else 0.25 * far
+    for t in range(C + N):  # scores: far * log 2 and 0 for queries of 1, between half and twice that for these
+        put(c, "k", 0, t, torch.full((D,), 96.0 if cache in (I8, E4M3) else low) * (t == 9), low)
+    put(c, "v", 0, 9, torch.zeros(D))
+    check(c, q, [C], sm_scale=0.6931 * 4 / D)
+
+
+@pytest.mark.parametrize("io", [F32, F16])
+def test_subnormal_elements_of_fp16_pages_count(gpu, io):
+    c = Cache(F16, 1, 1, 64, 16, 100, seed=3)
+    for x in (c.k, c.v):
+        x.copy_((x.float() * 2.0 ** -18).half())
+    q = 1000 * positive_rows(5, 4, 64, F32, torch.Generator().manual_seed(2))
+    got, want = check(c, q.to(io), [90], sm_scale=4.0)
+    assert want.abs().max() > 2.0 ** -21
+    if io == F32:
+        assert (got != 0).all()
