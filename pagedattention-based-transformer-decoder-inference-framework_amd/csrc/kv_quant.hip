@@ -20,7 +20,6 @@
 #include "paged_rows.hpp"
 
 #include <algorithm>
-#include <climits>
 
 namespace llm {
 namespace {
@@ -40,11 +39,6 @@ struct QuantArgs {
   int B, N;
   int tj_log, head_groups;  // a workgroup's tokens (log2), groups of heads
 };
-
-typedef _Float16 half8 __attribute__((ext_vector_type(8)));
-typedef __bf16 brain8 __attribute__((ext_vector_type(8)));
-typedef __bf16 brain2 __attribute__((ext_vector_type(2)));
-typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 template <typename T>
 __device__ __forceinline__ void load8(const void* base, long long at, float (&x)[kPer]) {
@@ -313,7 +307,7 @@ int quant(const char* name, const pa_kv_view* kv, const pa_kv_scales* scales, co
   const int heads = 1 << (rows_log - a.tj_log);
   a.head_groups = (H + heads - 1) / heads;
   const long long groups = (((long long)N + (1 << a.tj_log) - 1) >> a.tj_log) * a.head_groups;
-  LLM_REQUIRE(groups <= INT32_MAX / 64, who + "too many tokens in one call");
+  LLM_REQUIRE(groups < (1LL << 32) / kThreads, who + "too many tokens in one call");  // (threads of a launch)
   const dim3 grid((unsigned)groups, B);
   const bool i8 = kv->kv_dtype == LLM_I8;
   hipError_t e;
