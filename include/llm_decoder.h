@@ -376,7 +376,7 @@ typedef struct logits_rules {
  *   x = x - (frequency * c + presence * [c > 0])
  *   x = x + bias
  *   not allowed: x = -infinity
- * in fp32, rounded once at the end.  rows <= 65535. */
+ * in fp32, rounded once at the end.  rows <= 65535; V, history_len and bias_len <= 2^30. */
 int logits_adjust(const void* logits, void* out, int dtype, int rows, int V, long long stride,
                   const logits_rules* rules, void* stream);
 

@@ -13,13 +13,13 @@
 #include "paged_rows.hpp"
 
 #include <algorithm>
-#include <climits>
 
 namespace llm {
 namespace {
 
 constexpr int kThreads = 256;
 constexpr int kIds = 4;
+constexpr int kMostIds = 1 << 30;  // (places in a list and the steps behind it stay in 32 bits)
 constexpr uint32_t kPrompt = 0x80000000u;
 
 struct AdjustArgs {
@@ -194,12 +194,12 @@ extern "C" int logits_adjust(const void* logits, void* out, int dtype, int rows,
   LLM_REQUIRE((uintptr_t)logits % value_size(dtype) == 0 && (uintptr_t)out % value_size(dtype) == 0,
               "logits_adjust: logits and out must be aligned to their elements");
   const logits_rules& r = *rules;
-  LLM_REQUIRE(!r.history || (r.history_len >= 0 && (r.history_stride == 0 || r.history_stride >= r.history_len)),
+  LLM_REQUIRE(!r.history || (r.history_len >= 0 && r.history_len <= kMostIds && (r.history_stride == 0 || r.history_stride >= r.history_len)),
               "logits_adjust: bad history_len / history_stride");
   LLM_REQUIRE(r.history || (!r.repetition && !r.frequency && !r.presence),
               "logits_adjust: penalties need a history");
   LLM_REQUIRE(!r.bias_ids == !r.bias, "logits_adjust: bias_ids and bias go together");
-  LLM_REQUIRE(!r.bias_ids || (r.bias_len >= 0 && (r.bias_stride == 0 || r.bias_stride >= r.bias_len)),
+  LLM_REQUIRE(!r.bias_ids || (r.bias_len >= 0 && r.bias_len <= kMostIds && (r.bias_stride == 0 || r.bias_stride >= r.bias_len)),
               "logits_adjust: bad bias_len / bias_stride");
   LLM_REQUIRE(!r.allowed || r.num_masks > 0, "logits_adjust: num_masks must be positive");
   LLM_REQUIRE(!r.allowed || r.allowed_rows || r.num_masks >= rows,

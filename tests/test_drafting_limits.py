@@ -14,3 +14,15 @@ def test_more_tokens_than_a_launch_has_workgroups():
             assert call(view(), scales(), P, P, llm_capi.LLM_F16, 0, None, P, None, 1, N, None) == \
                 llm_capi.LLM_ERR_INVALID, N
             assert b"too many tokens" in lib.llm_last_error()
+
+
+def adjust(x=P, out=P, dtype=llm_capi.LLM_F32, rows=2, V=10, step=0, **rules):
+    return llm_capi.load().logits_adjust(x, out, dtype, rows, V, step, ctypes.byref(llm_capi.LogitsRules(**rules)),
+                                         None)
+
+
+def test_lists_that_a_thread_could_not_count_to():
+    """A thread steps 1024 entries at a time: past 2^31 - 1024 its place would leave 32 bits."""
+    for n in ((1 << 30) + 1, (1 << 31) - 1):
+        assert adjust(history=4096, history_len=n) == llm_capi.LLM_ERR_INVALID
+        assert adjust(bias_ids=4096, bias=4096, bias_len=n) == llm_capi.LLM_ERR_INVALID
