@@ -369,7 +369,7 @@ typedef struct logits_rules {
 /* Penalties for repeated tokens, biases and grammar masks, one pass over logits
  * [rows][V] of dtype (LLM_F32, LLM_F16 or LLM_BF16), `stride` elements from row
  * to row (0: V), into out of the same layout (out == logits: in place; other
- * overlaps are not allowed).  With c the times that token v is in its row's
+ * overlaps are refused).  With c the times that token v is in its row's
  * history behind the prompt and p whether it is in the prompt:
  *   x = logits[r][v]
  *   c > 0 or p:  x = x > 0 ? x / repetition : x * repetition

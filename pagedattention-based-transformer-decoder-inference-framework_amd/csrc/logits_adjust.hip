@@ -176,6 +176,16 @@ hipError_t launch_adjust(const AdjustArgs& a, int rows, hipStream_t st) {
                                                                            : launch_chunks<T, 1>(a, rows, st);
 }
 
+// Whether rows of V elements of `size` bytes at x and, elsewhere, at out share any: row by row, or one row of
+// the one with another of the other.
+bool rows_overlap(const void* x, const void* out, int size, int rows, int V, long long stride) {
+  const __int128 apart = (__int128)(intptr_t)out - (intptr_t)x, step = (__int128)stride * size;
+  const __int128 extent = step * (rows - 1) + (__int128)V * size;
+  if (apart == 0 || apart >= extent || -apart >= extent) return false;
+  const __int128 behind = (apart % step + step) % step;  // out's rows lie this far behind the next one of x
+  return behind < (__int128)V * size || step - behind < (__int128)V * size;
+}
+
 }  // namespace
 }  // namespace llm
 
@@ -193,6 +203,8 @@ extern "C" int logits_adjust(const void* logits, void* out, int dtype, int rows,
   LLM_REQUIRE(stride >= V, "logits_adjust: stride must be 0 or >= V");
   LLM_REQUIRE((uintptr_t)logits % value_size(dtype) == 0 && (uintptr_t)out % value_size(dtype) == 0,
               "logits_adjust: logits and out must be aligned to their elements");
+  LLM_REQUIRE(!rows_overlap(logits, out, value_size(dtype), rows, V, stride),
+              "logits_adjust: out must be the logits or not overlap them");
   const logits_rules& r = *rules;
   LLM_REQUIRE(!r.history || (r.history_len >= 0 && r.history_len <= kMostIds && (r.history_stride == 0 || r.history_stride >= r.history_len)),
               "logits_adjust: bad history_len / history_stride");

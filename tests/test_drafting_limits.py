@@ -26,3 +26,24 @@ def test_lists_that_a_thread_could_not_count_to():
     for n in ((1 << 30) + 1, (1 << 31) - 1):
         assert adjust(history=4096, history_len=n) == llm_capi.LLM_ERR_INVALID
         assert adjust(bias_ids=4096, bias=4096, bias_len=n) == llm_capi.LLM_ERR_INVALID
+
+
+def test_out_that_overlaps_the_logits():
+    """Rows of another place that share elements with the logits' rows; in place is not one of them."""
+    at = 1 << 20
+
+    def overlaps(by, rows=4, V=10, step=32):
+        # (with penalties that have no history: what does not overlap is refused for that)
+        assert adjust(x=ctypes.c_void_p(at), out=ctypes.c_void_p(at + by), rows=rows, V=V, step=step,
+                      repetition=4096) == llm_capi.LLM_ERR_INVALID
+        error = llm_capi.load().llm_last_error()
+        assert b"overlap" in error or b"history" in error
+        return b"overlap" in error
+
+    for by in (4, -4, 36, -36, 4 * 32, -4 * 32, 3 * 4 * 32 + 36, -(3 * 4 * 32 + 36), 4 * (2 * 32 - 9)):
+        assert overlaps(by), by
+    assert overlaps(4, rows=1) and overlaps(-36, rows=1) and overlaps(36, step=0)
+    # in place, beside the logits' rows, in the gaps between them, behind them
+    for by in (0, 40, -40, 88, 4 * 3 * 32 + 40, 4 * 4 * 32, -4 * 4 * 32, 4 * (32 + 10), 4 * (32 + 22)):
+        assert not overlaps(by), by
+    assert not overlaps(40, rows=1) and not overlaps(160, step=0)
