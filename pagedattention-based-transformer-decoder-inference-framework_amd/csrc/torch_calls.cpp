@@ -245,6 +245,8 @@ py::object adjust(const Tensor& logits, const MaybeTensor& history, const MaybeT
   if (allowed) {
     value(allowed->dim() == 2 && allowed->size(1) == (V + 31) / 32 && allowed->size(0) <= INT32_MAX,
           "allowed must be [masks][ceil(V / 32)]");
+    // (a list of no masks has no address, by which the library would take it for none asked for)
+    value(allowed_rows || allowed->size(0) >= R, "without allowed_rows every row needs a mask of its own in allowed");
     r.num_masks = (int)allowed->size(0);
   }
   r.allowed = reinterpret_cast<const uint32_t*>(ints(allowed, dev, {}, "allowed"));
