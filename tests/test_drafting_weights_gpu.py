@@ -33,14 +33,14 @@ def put(c, name, b, pos, codes, scale=None):
         c.scales["kv".index(name)][at] = scale
 
 
-def attention(q, c, contexts, mask, sm_scale):
+def attention(q, c, contexts, mask, sm_scale, beams=None):
     """(results, room) in 64 bits of chains or masks [B][N][N], one key head: q [B][N][H][D]."""
     B, N, H, D = q.shape
     out, room = torch.zeros(q.shape, dtype=torch.float64), torch.zeros(q.shape, dtype=torch.float64)
     for b in range(B):
         L = contexts[b] + N
-        k, ok = c.held("k", b, 0, L)
-        v, _ = c.held("v", b, 0, L)
+        k, ok = c.held("k", beams[b] if beams else b, 0, L)
+        v, _ = c.held("v", beams[b] if beams else b, 0, L)
         j = torch.arange(L) - contexts[b]
         for i in range(N):
             own = torch.arange(N) <= i if mask is None else mask[b, i]
@@ -197,3 +197,46 @@ def test_subnormal_elements_of_fp16_pages_count(gpu, io):
     assert want.abs().max() > 2.0 ** -21
     if io == F32:
         assert (got != 0).all()
+
+
+NOT_NUMBERS = [  # beams, B, N, H, contexts of the beams: one tile in parts, by 8 waves, four tiles, eight
+    (2, 2, 5, 2, [3060, 126]),
+    (4, 64, 2, 2, [700, 638, 900, 520]),
+    (1, 1, 30, 2, [3060]),
+    (1, 1, 70, 2, [3060]),
+]
+
+
+@pytest.mark.parametrize("cache", [F16, BF16, I8, E4M3])
+@pytest.mark.parametrize("io", [F32, BF16])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("form", range(len(NOT_NUMBERS)))
+def test_drafts_that_are_not_numbers(gpu, cache, io, D, form):
+    """A NaN in the second drafted token's values, infinities in the last one's: the rows that see them have what
+    the formula gives, in those dims alone, the others their own results."""
+    beams, B, N, H, contexts = NOT_NUMBERS[form]
+    g = torch.Generator().manual_seed(D + form)
+    c = Cache(cache, beams, 1, D, 16, max(contexts) + N, seed=form)
+    for b in range(beams):
+        second, last = c.slot(b, 0, contexts[b] + 1), c.slot(b, 0, contexts[b] + N - 1)
+        if cache == I8:
+            c.scales[1][second] = float("nan")
+            c.v[last][7] = 0
+        elif cache == E4M3:
+            c.v.view(torch.uint8)[second][3] = 0xff
+        else:
+            c.v[second][3] = float("nan")
+            c.v[last][5], c.v[last][6] = float("inf"), -float("inf")
+        if c.scales is not None and N > 2:
+            c.scales[1][last] = -float("inf")
+    ids = [b % beams for b in range(B)]
+    of_rows = [contexts[i] for i in ids]
+    q = torch.randn((B, N, H, D), generator=g).to(io)
+    d = c.cuda()
+    got = llm_capi.pa_tree(q.cuda(), d.k, d.v, d.table, T=max(contexts), context_lens=i32(of_rows), beam_ids=i32(ids),
+                           scales=d.scales, sm_scale=D ** -0.5).cpu()
+    want, room = attention(q, c, of_rows, None, D ** -0.5, ids)
+    fine = torch.isfinite(want)
+    assert fine[:, 0].all() and not fine[:, 1:].all(-1).any()
+    assert torch.equal(got[~fine].double().nan_to_num(7.0), want[~fine].nan_to_num(7.0))
+    close(torch.where(fine, got, 0), torch.where(fine, want, 0), torch.where(fine, room, 0), io)
