@@ -232,8 +232,9 @@ typedef struct pa_kv_scales {
  * scale NaN and codes 0.  A token whose position is negative or has no page is
  * left out, as is one whose beam id the page table does not have.  Where rows of
  * one beam overlap, the later row's token is kept.  Pages that two heads or
- * beams share are the caller's to part before they are written (as
- * kv_cache_fork's are by its copy-on-write).
+ * beams share are the caller's to part before they are written, with their
+ * scales: this call writes into the pages that the table has, and the copies that
+ * kv_cache_write_tokens makes of a forked beam's pages are of the pools alone.
  * head_dim a multiple of 8 up to 256; pools, k and v 16-byte aligned, and
  * token_stride a multiple of 16 bytes.  B <= 65535. */
 int kv_quant_write(const pa_kv_view* kv, const pa_kv_scales* scales, const void* k, const void* v,
@@ -265,7 +266,10 @@ int kv_quant_read(const pa_kv_view* kv, const pa_kv_scales* scales, void* k, voi
  * tokens (context_lens then counts the tokens ahead of it).
  * kv->kv_dtype LLM_F16 or LLM_BF16 (scales NULL), LLM_I8 (scales NULL: raw
  * values) or LLM_E4M3 with scales; D 64, 128 or 256; page_size a multiple of
- * 16; N <= 1024; H / num_heads <= 64; rows of q and out 16-byte aligned.  T is a
+ * 16; N <= 1024; H / num_heads <= 64; B <= 65535; B * num_heads and B * N * H below
+ * 2^23; rows of q and out 16-byte aligned.  Scores are numbers up to 2^23 in magnitude,
+ * keys of quantised pools up to 2^100; what is infinite among committed values makes its
+ * dims infinite or NaN.  T is a
  * bound on the committed tokens that sizes the launch; longer contexts are read
  * in full all the same.
  * Scores, sums and the output are accumulated in fp32, queries and probabilities enter
