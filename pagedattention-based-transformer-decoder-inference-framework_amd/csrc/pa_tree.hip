@@ -102,29 +102,50 @@ void plan_one_tile(TreePlan& p, const pa_kv_view& kv, long long base, long long 
 
 // Splits of more tiles, whose turns are long: the length for which one or two rounds of workgroups, or
 // whole rows, are priced least.  In us, as measured: a workgroup 8 and a turn of its KW blocks 2 (1.4 with
-// one tile a wave, 3.5 of heads of 256), 0.65 of it with a CU to itself; two a CU, three of heads of 64 in 8
-// bits with more than 64 rows; a merge 4.5, and every part's way through memory.  The rows of a batch of
-// 4 and more are taken to need 0.6 of T's splits.  (us, whole rows | one round | two: 24 x 16 x 40 rows of
-// 64 over up to 418 int8 tokens 18 | 32 | 36; 16 x 2 x 168 over 4096 bf16 - | 39 | 38; 26 x 228 of 64 over
-// 13,805 int8 149 | 83 | 60; 16 x 63 over 32768 e4m3 - | 55 | 67; 2 x 16 x 40 over 4800 fp16 - | 24 | 31;
-// 49 x 2 x 36 over 610 e4m3 23.4 | 17.7.)
+// one tile a wave, 3.5 of heads of 256), 0.65 of it with a CU to itself and up to that with every place taken;
+// two a CU, three of heads of 64 in 8 bits with more than 64 rows; a merge 4.5, and every part's way through
+// memory.  The plan does not know the rows' lengths.  From 4 rows on it prices two batches, one whose rows are
+// all as long as T and one whose rows have 0.6 of it on average, each relative to its own best, the uneven one,
+// which is what a server has, twice.  (us, even | uneven: 4 x 16 x 63 rows over 8192 int8 tokens in 13 parts, as the
+// uneven batch alone has it, 73 | 63, in 8 65 | 62; 64 x 4 x 40 over 2048 fp16 in 3 74 | 47, in 2 62 | 42;
+// 6 x 8 x 48 over 3000 fp16 in 12 38 | 27, in 8 31 | 27; 8 x 8 x 128 over 4096 fp16 in 11 76 | 51, in 7 63 | 57; 4 x 2 x
+// 2048 over 1024 bf16 in 6 71 | 80, in 4 66 | 62; 32 x 8 x 63 of 64 over 6000 int8 in 3 119 | 96, in 2 105 | 102.  Left
+// as the uneven batch has it: 16 x 2 x 168 over 4096 bf16 in 11 58 | 40, in 7 47 | 44.)
 void plan_tiles(TreePlan& p, const pa_kv_view& kv, int parts, int B, int N, int H, long long base, long long keys) {
   const int D = kv.head_dim, mt = tree_wave_tiles(D, parts);
   const int turn_keys = kTreeKeys * (mt == 2 && p.tiles == 4 ? 2 : 1);
-  const double share = B >= 4 ? 0.6 : 1.0, turn = D == 256 ? 3.5 : mt == 2 ? 2.0 : 1.4;
+  const double turn = D == 256 ? 3.5 : mt == 2 ? 2.0 : 1.4;
   const double slots = D == 256 ? 256 : D == 64 && paged_elem_size(kv.kv_dtype) == 1 && p.tiles == 8 ? 768 : 512;
-  const double part = (double)B * N * H * share * (D + 2) * 8 / 3.5e6;
-  double least = 0;
-  for (int rounds = 0; rounds <= 2; ++rounds) {
-    const long long n = rounds ? std::max(1LL, (long long)(rounds * slots / (share * base))) : 1;
-    const long long per = std::max(128LL, ((keys + n - 1) / n + kTreeStep - 1) / kTreeStep * kTreeStep);
-    const long long m = (keys + per - 1) / per;
-    const double groups = m > 1 ? share * base * m : (double)base;
-    const double one = 8 + (double)std::min(per, keys) / turn_keys * turn * (groups <= 256 ? 0.65 : 1.0);
-    const double cost = std::ceil(groups / slots) * one + (m > 1 ? 4.5 + part * m : 0);
-    if (rounds && cost >= least) continue;
+  const double part = (double)B * N * H * (D + 2) * 8 / 1.2e7;
+  // rows of `share` of the longest row's splits (and of a last one that is not full, 0.25 more)
+  auto price = [&](long long per, double share) {
+    const double m = (double)((keys + per - 1) / per);
+    const double groups = base * (share < 1 ? std::min(m, share * m + 0.25) : m);
+    const double turns = (double)std::min(per, keys) / turn_keys * turn;
+    const double full = std::floor(groups / slots), rest = groups / slots - full;
+    return full * (8 + turns) + (rest > 0 ? 8 + turns * (0.65 + 0.35 * std::max(2 * rest - 1, 0.0)) : 0) +
+           (m > 1 ? 4.5 + part * share * m : 0);
+  };
+  constexpr double kShares[2] = {1.0, 0.6}, kWeights[2] = {1.0, 2.0};
+  const int batches = B >= 4 ? 2 : 1;
+  long long pers[5];
+  int n = 0;
+  for (int rounds = 0; rounds <= 2; ++rounds)
+    for (int i = 0; i < (rounds ? batches : 1); ++i) {
+      const long long want = rounds ? std::max(1LL, (long long)(rounds * slots / (kShares[i] * base))) : 1;
+      pers[n++] = std::max(128LL, ((keys + want - 1) / want + kTreeStep - 1) / kTreeStep * kTreeStep);
+    }
+  double best[2], least = 0;
+  for (int i = 0; i < batches; ++i) {
+    best[i] = price(pers[0], kShares[i]);
+    for (int c = 1; c < n; ++c) best[i] = std::min(best[i], price(pers[c], kShares[i]));
+  }
+  for (int c = 0; c < n; ++c) {
+    double cost = 0;
+    for (int i = 0; i < batches; ++i) cost += kWeights[i] * price(pers[c], kShares[i]) / best[i];
+    if (c && cost >= least) continue;
     least = cost;
-    p.split_keys = (int)std::min(per, 1LL << 30);
+    p.split_keys = (int)std::min(pers[c], 1LL << 30);
   }
 }
 

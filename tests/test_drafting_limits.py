@@ -47,3 +47,22 @@ def test_out_that_overlaps_the_logits():
     for by in (0, 40, -40, 88, 4 * 3 * 32 + 40, 4 * 4 * 32, -4 * 4 * 32, 4 * (32 + 10), 4 * (32 + 22)):
         assert not overlaps(by), by
     assert not overlaps(40, rows=1) and not overlaps(160, step=0)
+
+
+def parts_of(B, N, heads, group, D, T, kv_dtype):
+    """Parts that long rows are taken in, from what the call asks for them."""
+    H = heads * group
+    v = view(num_heads=heads, head_dim=D, kv_dtype=kv_dtype, max_tiles=4096)
+    size = llm_capi.load().pa_tree_workspace_bytes(v, B, N, H, T)
+    assert size % (B * N * H * (D + 2) * 4) == 0
+    return size // (B * N * H * (D + 2) * 4)
+
+
+def test_parts_of_batches_that_may_be_even():
+    """Batches for which a plan for uneven rows alone has half a round too many when all are of one length, and
+    gains nothing for it when they are not."""
+    I8, F16, BF16 = llm_capi.LLM_I8, llm_capi.LLM_F16, llm_capi.LLM_BF16
+    for most, batch in ((8, (4, 63, 16, 1, 128, 8192, I8)), (2, (64, 5, 4, 8, 128, 2048, F16)),
+                        (8, (6, 24, 8, 2, 128, 3000, F16)), (7, (8, 128, 8, 1, 128, 4096, F16)),
+                        (4, (4, 512, 2, 4, 128, 1024, BF16))):
+        assert 1 < parts_of(*batch) <= most, batch
