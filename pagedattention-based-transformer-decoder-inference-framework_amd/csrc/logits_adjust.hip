@@ -167,7 +167,8 @@ hipError_t launch_chunks(const AdjustArgs& a, int rows, hipStream_t st) {
 // (64 rows of 50,257 fp32 tokens, history 4096: 12.0 us, by one load 13.4; 336 of 32,768 bf16
 // 15.6 and 15.7), one where the rows are few (one row of 50,257: 3.1, by two 3.5) or both lists take LDS
 // from 16-bit rows, whose chunks are twice as long (256 of 50,257 bf16 with biases: 18.5, by two 23.0).
-// An empty launch is 2 us of these; the bytes alone are 5.5, 9.6 and 10.8 at the rate of a copy.
+// An empty launch is 2 us of these, which are between the host's events (a profiler's clock has 12.0 and 16.4
+// for the first two); the bytes alone are 5.5, 9.6 and 10.8 at the rate of a copy.
 template <typename T>
 hipError_t launch_adjust(const AdjustArgs& a, int rows, hipStream_t st) {
   constexpr int CHUNK = chunk_of<T, 2>();

@@ -27,11 +27,12 @@
 // are bf16, which has fp32's range.
 //
 // What bounds it: one tile, the memory (64 x 16 heads of 128 over up to 8192 int8 tokens, pages of 2 KB and
-// their scales in any order: 231 us, 5.2 TB/s; with the products left out 225); more tiles, a
-// SIMD's instructions, of which the scores' exponentials and scales are half (16 heads x 63 rows over 32768
-// e4m3 tokens: 54 us, 2.6 TB/s and 310 TFLOP/s; 16 x 2 x 168 rows over up to 4096 bf16: 33 us): tiles of sums,
-// queries and a block fill the registers of two waves a SIMD.  Short rows, a launch and its code (8 rows of
-// 12 heads over 113 tokens: 5.6 us).
+// their scales in any order: 241 us, 5.1 TB/s, vector instructions 43 % of it).  More tiles, the chain of one
+// block (loads, scores, exponentials, products), which too few waves hide: 16 heads x 63 rows over 32768 e4m3 tokens
+// 57 us, 2.4 TB/s and 300 TFLOP/s, with 1.3 waves a SIMD whose vector instructions take 42 % of the time and
+// its products 17 %; 16 x 2 x 168 rows over up to 4096 bf16 33 us, where 278 of 704 workgroups have keys:
+// 0.7 waves a SIMD, 16 % and 7 %.  Tiles of sums, queries and a block fill the registers of two waves a
+// SIMD.  Short rows, a launch and its code (8 rows of 12 heads over 113 tokens: 5.6 us).
 //
 // Keys that a row does not see get the score -infinity.  Their V still meets a probability of 0
 // in the product, and 0 times NaN is NaN: rows of V that nobody sees (behind the row's end, in

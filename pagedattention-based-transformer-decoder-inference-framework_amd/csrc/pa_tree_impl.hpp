@@ -148,7 +148,7 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 8 / WAVES : 1) void pa_tree_
   const int lane = lane_id(), g = lane >> 4, c = lane & 15;
   const int w = wave_id_uniform(), kw = w % KW, rw = w / KW;
   // Workgroups go round the XCDs.  Staged, a pair's splits lie beside each other, so that a long row's are
-  // dealt out over all of them (16 x 2 pairs of 168 rows, 11 splits 55 -> 38 us); else the pairs do,
+  // dealt out over all of them (16 x 2 pairs of 168 rows, 11 splits 46.7 -> 39.5 us); else the pairs do,
   // which are many (64 x 16 pairs by splits 249 us, by pairs 241).
   const int pair = STAGED ? blockIdx.x / a.nsplit : blockIdx.x;
   const int split = STAGED ? blockIdx.x - pair * a.nsplit : blockIdx.y;
