@@ -240,3 +240,54 @@ def test_drafts_that_are_not_numbers(gpu, cache, io, D, form):
     assert fine[:, 0].all() and not fine[:, 1:].all(-1).any()
     assert torch.equal(got[~fine].double().nan_to_num(7.0), want[~fine].nan_to_num(7.0))
     close(torch.where(fine, got, 0), torch.where(fine, want, 0), torch.where(fine, room, 0), io)
+
+
+@pytest.mark.parametrize("cache", [F16, BF16, I8, E4M3])
+@pytest.mark.parametrize("N,H,D,C,T", [(3, 2, 128, [2500, 31], 2500), (33, 2, 64, [700, 700], 5000),
+                                       (5, 64, 128, [1, 200], 200), (100, 3, 256, [128], 1)])
+def test_wide_rows_bits_behind_the_tree_and_one_context(gpu, cache, N, H, D, C, T):
+    """q and out in wider rows (joined from parts as well), masks whose bits behind the last token are anything,
+    pools without scales, and every row at T."""
+    B = len(C)
+    g = torch.Generator().manual_seed(N + D)
+    c = Cache(cache, B, 1, D, 48, max(C) + N, seed=N)
+    if cache == I8:
+        c.scales = None
+    q = ((0.02 if cache == I8 else 1.5) * torch.randn((B, N, H, D), generator=g)).to(BF16)
+    words = -(-N // 32)
+    full = torch.rand((B, N, words * 32), generator=g) < 0.5
+    full[:, torch.arange(N), torch.arange(N)] = True
+    w = (full.long().view(B, N, words, 32) << torch.arange(32)).sum(-1)
+    w = torch.where(w >= 1 << 31, w - (1 << 32), w).to(torch.int32)
+    d = c.cuda()
+    wide = torch.full((2, B, N, H * D + 16), 3.25, dtype=BF16, device="cuda")
+    qd, out = (x[..., :H * D].unflatten(-1, (H, D)) for x in wide)
+    qd.copy_(q)
+    one = C[0] == T and len(set(C)) == 1
+    got = llm_capi.pa_tree(qd, d.k, d.v, d.table, T=T, context_lens=None if one else i32(C), tree_mask=w.cuda(),
+                           scales=d.scales, sm_scale=D ** -0.5, out=out)
+    assert (wide[:, ..., H * D:] == 3.25).all() and torch.equal(qd.cpu(), q)
+    want, room = attention(q, c, C, full[..., :N], D ** -0.5)
+    close(got, want, room, BF16)
+    if len(set(C)) == 1:
+        got = llm_capi.pa_tree(qd, d.k, d.v, d.table, T=C[0], tree_mask=w.cuda(), scales=d.scales, sm_scale=D ** -0.5)
+        close(got, want, room, BF16)
+
+
+def test_two_calls_at_once(gpu):
+    """Two streams with calls in parts, each with a workspace of its own, against the calls alone."""
+    c = Cache(I8, 2, 1, 128, 16, 2600, seed=1).cuda()
+    q = [torch.randn((2, n, 4, 128), generator=torch.Generator().manual_seed(n)).cuda() for n in (2, 30)]
+    call = lambda x: llm_capi.pa_tree(x, c.k, c.v, c.table, T=2500, context_lens=i32([2500, 1900]), scales=c.scales,
+                                      sm_scale=0.09)
+    want = [call(x) for x in q]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in q]
+    got = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(call(q[i]))
+    torch.cuda.synchronize()
+    for x, ys in zip(want, got):
+        assert all(torch.equal(x, y) for y in ys)
