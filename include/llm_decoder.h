@@ -273,9 +273,10 @@ int kv_quant_read(const pa_kv_view* kv, const pa_kv_scales* scales, void* k, voi
  * bound on the committed tokens that sizes the launch; longer contexts are read
  * in full all the same.
  * Scores, sums and the output are accumulated in fp32, queries and probabilities enter
- * their products in parts of 16 bits: queries of fp32 with 22 bits or more, probabilities (times
- * the value's scale) with 16 bits or more, for fp32 results 22.  Over fp16 pools a probability is
- * off by up to 2^-35 of the row's largest besides.  The workspace holds the
+ * their products in parts of 16 bits: queries of fp32 with 22 bits (or to 2^-39 of the row's
+ * largest element; over bf16 pools with all 24), probabilities, times the value's scale, with
+ * 16 bits or more, for fp32 results 22.  Over fp16 pools a probability is off by up to 2^-35 of
+ * the row's largest besides.  The workspace holds the
  * parts of long rows: pa_tree_workspace_bytes of the call's own arguments (a
  * shorter T may take more parts), 16-byte aligned, one for each call that may
  * run at the same time. */

@@ -702,63 +702,63 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 8 / WAVES : 1) void pa_tree_
     }
   }
   if (__any(unusable)) {
-      // The rows that see them get what the products left out: sums of ones count them.
-      for (int i = max((tr.C - lo) / (KW * kTreeKeys) - 1, 0); i < mine; ++i) {
-        const int key0 = lo + (i * KW + kw) * kTreeKeys;
-        if (key0 + kTreeKeys <= tr.C || key0 >= hi) continue;
-        look_up(key0 + 16 * (lane & 1));
-        const uint32_t present = present_of((uint32_t)__ballot(found) & 3u, key0);
-        u32x4 one[MT];
+    // The rows that see them get what the products left out: sums of ones count them.
+    for (int i = max((tr.C - lo) / (KW * kTreeKeys) - 1, 0); i < mine; ++i) {
+      const int key0 = lo + (i * KW + kw) * kTreeKeys;
+      if (key0 + kTreeKeys <= tr.C || key0 >= hi) continue;
+      look_up(key0 + 16 * (lane & 1));
+      const uint32_t present = present_of((uint32_t)__ballot(found) & 3u, key0);
+      u32x4 one[MT];
 #pragma unroll
-        for (int t = 0; t < MT; ++t) {
-          const uint32_t seen = present & visible(tok[t], key0);
+      for (int t = 0; t < MT; ++t) {
+        const uint32_t seen = present & visible(tok[t], key0);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t two = seen >> (16 * (e / 2) + 4 * g + 2 * (e % 2));
-            one[t][e] = (two & 1u ? Hf::kOne : 0u) | (two & 2u ? Hf::kOne << 16 : 0u);
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t two = seen >> (16 * (e / 2) + 4 * g + 2 * (e % 2));
+          one[t][e] = (two & 1u ? Hf::kOne : 0u) | (two & 2u ? Hf::kOne << 16 : 0u);
+        }
+      }
+#pragma unroll
+      for (int dd = 0; dd < ND; ++dd) {
+        u32x4 plus, minus;  // +infinity or NaN, -infinity or NaN
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          plus[e] = minus[e] = 0;
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            const int u = e / 2, key = 4 * g + 2 * (e % 2) + s;
+            if (!(present >> (16 * u + key) & 1u)) continue;
+            const uint8_t* at = a.v_pool + lane64(at_pool, u) + (uint32_t)(key * ROWB + (c * ND + dd) * ES);
+            const uint32_t x = ES == 1 ? *at : *reinterpret_cast<const uint16_t*>(at);
+            constexpr uint32_t kSign = ES == 1 ? 0x80u : 0x8000u;
+            bool bad = false, nan = false, minus_of = (x & kSign) != 0;
+            if constexpr (KVT != LLM_I8) {
+              constexpr uint32_t kInf = Unusable<KVT>::kInf;
+              bad = (x & kInf) == kInf, nan = ES == 1 ? bad : (x & (kSign - 1u)) > kInf;
+            }
+            if constexpr (QUANT)
+              if (a.v_scale) {
+                const float f = *reinterpret_cast<const float*>(reinterpret_cast<const uint8_t*>(a.v_scale) +
+                                                                lane64(at_scale, u) + 4 * key);
+                bad |= !(fabsf(f) < INFINITY);
+                nan |= f != f || !(KVT == LLM_I8 ? x : x & (kSign - 1u));  // (infinity times 0)
+                minus_of ^= f < 0.f;
+              }
+            if (bad && (nan || !minus_of)) plus[e] |= Hf::kOne << 16 * s;
+            if (bad && (nan || minus_of)) minus[e] |= Hf::kOne << 16 * s;
           }
         }
+        const f32x4 none = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int dd = 0; dd < ND; ++dd) {
-          u32x4 plus, minus;  // +infinity or NaN, -infinity or NaN
+        for (int t = 0; t < MT; ++t) {
+          const f32x4 up = Hf::dot(plus, one[t], none), down = Hf::dot(minus, one[t], none);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            plus[e] = minus[e] = 0;
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-              const int u = e / 2, key = 4 * g + 2 * (e % 2) + s;
-              if (!(present >> (16 * u + key) & 1u)) continue;
-              const uint8_t* at = a.v_pool + lane64(at_pool, u) + (uint32_t)(key * ROWB + (c * ND + dd) * ES);
-              const uint32_t x = ES == 1 ? *at : *reinterpret_cast<const uint16_t*>(at);
-              constexpr uint32_t kSign = ES == 1 ? 0x80u : 0x8000u;
-              bool bad = false, nan = false, minus_of = (x & kSign) != 0;
-              if constexpr (KVT != LLM_I8) {
-                constexpr uint32_t kInf = Unusable<KVT>::kInf;
-                bad = (x & kInf) == kInf, nan = ES == 1 ? bad : (x & (kSign - 1u)) > kInf;
-              }
-              if constexpr (QUANT)
-                if (a.v_scale) {
-                  const float f = *reinterpret_cast<const float*>(reinterpret_cast<const uint8_t*>(a.v_scale) +
-                                                                  lane64(at_scale, u) + 4 * key);
-                  bad |= !(fabsf(f) < INFINITY);
-                  nan |= f != f || !(KVT == LLM_I8 ? x : x & (kSign - 1u));  // (infinity times 0)
-                  minus_of ^= f < 0.f;
-                }
-              if (bad && (nan || !minus_of)) plus[e] |= Hf::kOne << 16 * s;
-              if (bad && (nan || minus_of)) minus[e] |= Hf::kOne << 16 * s;
-            }
-          }
-          const f32x4 none = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int t = 0; t < MT; ++t) {
-            const f32x4 up = Hf::dot(plus, one[t], none), down = Hf::dot(minus, one[t], none);
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              o[t][dd][r] += (up[r] > 0.f ? INFINITY : 0.f) - (down[r] > 0.f ? INFINITY : 0.f);
-          }
+          for (int r = 0; r < 4; ++r)
+            o[t][dd][r] += (up[r] > 0.f ? INFINITY : 0.f) - (down[r] > 0.f ? INFINITY : 0.f);
         }
       }
     }
+  }
 
   // The sums of a tile's waves, relative to the largest maximum of the row.
   // a row, ND of its dims; the first 256 threads take a tile, the others the next
